@@ -251,6 +251,115 @@ int s2b_linear(s2b_ctx* ctx, const float* x, int M, int K, const float* W, int N
 int s2b_linear_bf16_dev(s2b_ctx* ctx, const void* d_x, int M, int K, const void* d_w, int N, const float* d_bias,
                         void* d_y, void* stream);
 
+/* ---- operators beside the DiT ----------------------------------------- */
+/* No counterpart in the reference.  What stands around the DiT's Linears and
+ * attention when they run in 8 bits, over other geometries than its windows,
+ * or between the VAE's blocks: 8-bit block quantisation, the 8-bit Linear,
+ * rotary positions and GroupNorm.  Common rules:
+ *   - element types are S2B_PREC_FP32, _FP16 or _BF16; pitches and strides are
+ *     in elements; buffers are memory of the context's device (S2B_ERR_ARG for
+ *     host memory or another device's), aligned to their type;
+ *   - arguments are checked before anything else, with a null context too
+ *     (the message is then in s2b_last_error(NULL));
+ *   - calls enqueue on `stream` and return; they allocate nothing, keep
+ *     nothing and can be captured into a graph; the caller's current device
+ *     stays what it was;
+ *   - a call with no rows (or tokens, heads, columns) to write is S2B_OK and
+ *     writes nothing; no call writes outside the rows x columns it names;
+ *   - results do not depend on timing: the same call gives the same bits. */
+
+/* 8-bit codes (e4m3: 4 exponent bits, 3 fraction bits, largest 448) of x
+ * (rows, cols), with one scale for each block of 128 columns x block_rows rows;
+ * block_rows is 1 (activations) or 128 (weights).  The scale is 2^k with the
+ * smallest k >= -126 for which the block's largest finite |x| <= 448 * 2^k, and
+ * a code is x / 2^k rounded to the nearest code, ties to even; NaN and
+ * infinities become the code's NaN.  Blocks at the right and lower edge hold
+ * what is left.  q is (rows, cols) bytes of row pitch ldq (a multiple of 16;
+ * base 16-byte aligned).  Scales, dense: block_rows 1: [ceil(cols / 128)][rows];
+ * 128: [ceil(rows / 128)][ceil(cols / 128)]. */
+int s2b_fp8_quant_dev(s2b_ctx* ctx, const void* d_x, int x_type, int rows, int cols, int ldx, int block_rows,
+                      void* d_q, int ldq, float* d_scale, void* stream);
+/* The Linear on 8-bit operands, on the tcgen05 tensor cores:
+ *   y[m, n] = sum_b xs[b][m] * ws[n / 128][b] * sum_{k in block b} xq[m, k] * wq[n, k] + bias[n]
+ * xq (M, K) and wq (N, K) e4m3 codes with row pitches ldx, ldw in bytes
+ * (multiples of 16, bases 16-byte aligned), scales laid out as
+ * s2b_fp8_quant_dev writes them for block_rows 1 and 128; they may be any fp32
+ * values whose product is one (0 and powers of two included), from any
+ * quantiser.  bias (N) or NULL.  y (M, N) of y_type, row pitch ldy.  Any M, N,
+ * K > 0; one row to thousands.  Sums are fp32, rounded once to y_type; a NaN
+ * code makes the outputs that it enters NaN.  y must not overlap an operand.
+ * A bounded wait that expires is reported by s2b_check_errors. */
+int s2b_linear_fp8_dev(s2b_ctx* ctx, const void* d_xq, int ldx, const float* d_xs, int M, int K, const void* d_wq,
+                       int ldw, const float* d_ws, int N, const float* d_bias, void* d_y, int y_type, int ldy,
+                       void* stream);
+
+/* Rotary positions.  Pair i < pairs of a head turns by the angle
+ * pos[axis(i)] * f_i:  (a, b) -> (a cos - b sin, a sin + b cos) * amplitude.
+ * Interleaved pairs are (2i, 2i + 1), as the DiT's own RoPE has them
+ * (src/dit_vk.cpp:62-71); half pairs are (i, i + pairs).  Values past the
+ * 2 * pairs rotated ones are copied.  The pairs go to 1 to 3 axes in turn,
+ * axis a taking axis_dim[a] / 2 of them with f_j = theta^(-2 j / axis_dim[a])
+ * (the DiT: 3 axes of 42 dims, theta 10000, src/awa_window.cpp:15-150).
+ * Scalings for streams longer than the model was trained on:
+ *   NONE    f_j
+ *   LINEAR  f_j / factor
+ *   NTK     theta * factor^(d / (d - 2)) in theta's place (d = axis_dim)
+ *   YARN    f_j for pairs that turn more than beta_fast times over
+ *           original_length positions, f_j / factor below beta_slow, a linear
+ *           ramp over j between; amplitude 0.1 ln(factor) + 1 (else 1) */
+#define S2B_ROPE_INTERLEAVED 0
+#define S2B_ROPE_HALF 1
+#define S2B_ROPE_SCALE_NONE 0
+#define S2B_ROPE_SCALE_LINEAR 1
+#define S2B_ROPE_SCALE_NTK 2
+#define S2B_ROPE_SCALE_YARN 3
+#define S2B_ROPE_MAX_PAIRS 128
+typedef struct s2b_rope_config {
+    int layout, axes, axis_dim[3];   /* axis_dim: even, together at most 256 */
+    double theta;
+    int scaling;
+    double factor;                   /* >= 1 (LINEAR, NTK, YARN) */
+    double original_length, beta_fast, beta_slow;   /* YARN */
+} s2b_rope_config;
+/* Made by s2b_rope_plan, passed by value into the kernels: plain host memory. */
+typedef struct s2b_rope {
+    int pairs, half, axes;
+    float amplitude;
+    uint64_t turns[S2B_ROPE_MAX_PAIRS];   /* f_i / 2 pi as a 64-bit fraction of a turn */
+    uint8_t axis[S2B_ROPE_MAX_PAIRS];
+} s2b_rope;
+/* Host only, no context; messages in s2b_last_error(NULL). */
+int s2b_rope_plan(const s2b_rope_config* config, s2b_rope* plan);
+/* y = x with the heads turned (inverse 0) or turned back (inverse not 0: the
+ * transposed map, amplitude included, which is the gradient's).  Head h of
+ * token t of sample b starts at x + b * x_strides[0] + t * x_strides[1] +
+ * h * x_strides[2] and holds head_dim adjacent values (head_dim >= 2 * pairs);
+ * y likewise.  Position of a token on axis a: d_pos[b * pos_batch_stride +
+ * t * axes + a] (int32, any value; stride 0 shares them between samples), or
+ * pos0 + t on every axis when d_pos is NULL.  y may be x with the same strides;
+ * otherwise the two must not overlap.  Angles are exact to 2^-32 of a turn at
+ * every position. */
+int s2b_rope_dev(s2b_ctx* ctx, const s2b_rope* plan, const void* d_x, int type, int batch, int tokens, int heads,
+                 int head_dim, const long x_strides[3], const int* d_pos, long pos_batch_stride, int pos0, void* d_y,
+                 const long y_strides[3], int inverse, void* stream);
+
+/* GroupNorm over channel-last rows, with an activation:
+ *   y = act((x - mean_g) / sqrt(var_g + eps) * gamma[c] + beta[c])
+ * with the mean and (biased) variance over the rows and the channels / groups
+ * adjacent channels of group g of one sample; statistics in fp32.  x is
+ * (batch, rows, channels) with row pitch ldx (samples adjacent), y likewise
+ * with ldy; gamma, beta (channels) fp32 or NULL (1, 0).  y may be x with the
+ * same type and pitch; otherwise they must not overlap.  d_work: device
+ * workspace of s2b_groupnorm_workspace bytes (16-byte aligned), contents
+ * arbitrary before and after; two calls that may run at the same time need one
+ * each. */
+#define S2B_ACT_NONE 0
+#define S2B_ACT_SILU 1
+int s2b_groupnorm_workspace(int batch, int rows, int channels, int groups, size_t* bytes);
+int s2b_groupnorm_dev(s2b_ctx* ctx, const void* d_x, int x_type, int batch, int rows, int channels, int ldx,
+                      int groups, const float* d_gamma, const float* d_beta, float eps, int act, void* d_y, int y_type,
+                      int ldy, void* d_work, size_t work_bytes, void* stream);
+
 /* ---- synthetic data (no checkpoint ships with this build) ------------- */
 /* Writes the m5 directory layout for layers [layer_lo, layer_hi) with
  * seeded random-init weights (Linear N(0,0.02) stored fp16; biases and
@@ -330,7 +439,7 @@ int s2b_shard_plan(const s2b_win* ns, const s2b_win* sh, int world, int rank, in
  * stream, then returns S2B_ERR_TIMEOUT (and clears the status) if a bounded
  * wait expired in any of them since the last report, else S2B_OK.  Calls that
  * run on the caller's stream (s2b_awa_forward_dev, s2b_awa_forward_dev_static,
- * s2b_linear_bf16_dev) must be complete first (synchronise that stream).  The
+ * s2b_linear_bf16_dev, s2b_linear_fp8_dev) must be complete first (synchronise that stream).  The
  * reference reports failures of its GPU work through the return value of each
  * synchronous call (src/awa_vk.cpp:182, src/dit_vk.cpp:27-45); this is the
  * same report for the stream-ordered form. */

@@ -2,6 +2,7 @@
 #include "../../include/seedvr2_b200.h"
 #include "dit_b200.h"
 #include "dit_shard.h"
+#include "ops.h"
 #include "synth.h"
 #include "shard_plan.h"
 #include <cstring>
@@ -34,6 +35,54 @@ int to_geom(const s2b_win* w, s2b::WinGeom& g, std::string& err) {
     if ((w->n_vid_freq && !w->vid_freq) || (w->n_txt_freq && !w->txt_freq)) { err = "null freq tables"; return S2B_ERR_ARG; }
     g.vid_freq.assign(w->vid_freq, w->vid_freq + w->n_vid_freq);
     g.txt_freq.assign(w->txt_freq, w->txt_freq + w->n_txt_freq);
+    return S2B_OK;
+}
+
+// Refuses an operator call: the message goes where s2b_last_error(ctx) looks.
+int refuse(s2b_ctx* ctx, int code, const char* why) {
+    (ctx ? ctx->dit.err : g_create_err) = why;
+    return code;
+}
+
+// Restores the caller's current device.
+struct DeviceScope {
+    int prev = -1;
+    cudaError_t enter(int dev) {
+        cudaError_t e = cudaGetDevice(&prev);
+        if (e != cudaSuccess || prev == dev) { prev = -1; return e; }
+        return cudaSetDevice(dev);
+    }
+    ~DeviceScope() { if (prev >= 0) cudaSetDevice(prev); }
+};
+
+// The operators beside the DiT: arguments are checked before the context is
+// looked at, buffers have to be memory of the context's device, the kernels
+// are enqueued on `stream` with that device current.
+template <class Args>
+int run_op(s2b_ctx* ctx, const Args& a, void* stream) {
+    if (const char* why = s2b::op_check(a)) return refuse(ctx, S2B_ERR_ARG, why);
+    if (!ctx) return refuse(ctx, S2B_ERR_ARG, "null context");
+    if (s2b::op_empty(a)) return S2B_OK;
+    const int dev = ctx->dit.device();
+    DeviceScope scope;
+    if (scope.enter(dev) != cudaSuccess) return refuse(ctx, S2B_ERR_CUDA, "the context's device cannot be made current");
+    const s2b::OpPtrs ptrs = s2b::op_ptrs(a);
+    for (int i = 0; i < ptrs.n; i++) {
+        if (!ptrs.p[i]) continue;
+        cudaPointerAttributes at;
+        if (cudaPointerGetAttributes(&at, ptrs.p[i]) != cudaSuccess) {
+            cudaGetLastError();
+            return refuse(ctx, S2B_ERR_ARG, "a buffer is not device memory");
+        }
+        if (!((at.type == cudaMemoryTypeDevice && at.device == dev) || at.type == cudaMemoryTypeManaged))
+            return refuse(ctx, S2B_ERR_ARG, "a buffer is not memory of the context's device");
+    }
+    cudaGetLastError();                  // an earlier call's error is not this one's
+    const int n = s2b::op_launch(a, (cudaStream_t)stream);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return refuse(ctx, S2B_ERR_CUDA, cudaGetErrorString(e));
+    if (n < 0) return refuse(ctx, S2B_ERR_UNSUPPORTED, "the operator's kernel cannot be launched for this call");
+    ctx->dit.count_launches(n);
     return S2B_OK;
 }
 }  // namespace
@@ -281,6 +330,46 @@ int s2b_linear_bf16_dev(s2b_ctx* ctx, const void* d_x, int M, int K, const void*
                         void* d_y, void* stream) {
     if (!ctx) return S2B_ERR_ARG;
     return ctx->dit.linear_bf16_dev(d_x, M, K, d_w, N, d_bias, d_y, (cudaStream_t)stream);
+}
+
+int s2b_fp8_quant_dev(s2b_ctx* ctx, const void* d_x, int x_type, int rows, int cols, int ldx, int block_rows, void* d_q,
+                      int ldq, float* d_scale, void* stream) {
+    return run_op(ctx, s2b::Fp8QuantArgs{d_x, x_type, rows, cols, ldx, block_rows, d_q, ldq, d_scale}, stream);
+}
+
+int s2b_linear_fp8_dev(s2b_ctx* ctx, const void* d_xq, int ldx, const float* d_xs, int M, int K, const void* d_wq, int ldw,
+                       const float* d_ws, int N, const float* d_bias, void* d_y, int y_type, int ldy, void* stream) {
+    return run_op(ctx, s2b::Fp8LinearArgs{d_xq, ldx, d_xs, M, K, d_wq, ldw, d_ws, N, d_bias, d_y, y_type, ldy}, stream);
+}
+
+int s2b_rope_plan(const s2b_rope_config* config, s2b_rope* plan) {
+    if (!config || !plan) return refuse(nullptr, S2B_ERR_ARG, "rope plan: null argument");
+    if (const char* why = s2b::rope_plan(*config, plan)) return refuse(nullptr, S2B_ERR_ARG, why);
+    return S2B_OK;
+}
+
+int s2b_rope_dev(s2b_ctx* ctx, const s2b_rope* plan, const void* d_x, int type, int batch, int tokens, int heads,
+                 int head_dim, const long x_strides[3], const int* d_pos, long pos_batch_stride, int pos0, void* d_y,
+                 const long y_strides[3], int inverse, void* stream) {
+    if (!x_strides || !y_strides) return refuse(ctx, S2B_ERR_ARG, "rope: null strides");
+    return run_op(ctx, s2b::RopeArgs{plan, d_x, type, batch, tokens, heads, head_dim,
+                                     {x_strides[0], x_strides[1], x_strides[2]}, d_pos, pos_batch_stride, pos0, d_y,
+                                     {y_strides[0], y_strides[1], y_strides[2]}, inverse}, stream);
+}
+
+int s2b_groupnorm_workspace(int batch, int rows, int channels, int groups, size_t* bytes) {
+    if (!bytes) return refuse(nullptr, S2B_ERR_ARG, "groupnorm: null argument");
+    if (batch < 0 || rows < 0 || channels <= 0 || groups <= 0)
+        return refuse(nullptr, S2B_ERR_ARG, "groupnorm: batch and rows must not be negative, channels and groups must be positive");
+    *bytes = s2b::groupnorm_workspace(batch, rows, channels, groups);
+    return S2B_OK;
+}
+
+int s2b_groupnorm_dev(s2b_ctx* ctx, const void* d_x, int x_type, int batch, int rows, int channels, int ldx, int groups,
+                      const float* d_gamma, const float* d_beta, float eps, int act, void* d_y, int y_type, int ldy,
+                      void* d_work, size_t work_bytes, void* stream) {
+    return run_op(ctx, s2b::GroupNormArgs{d_x, x_type, batch, rows, channels, ldx, groups, d_gamma, d_beta, eps, act,
+                                          d_y, y_type, ldy, d_work, work_bytes}, stream);
 }
 
 int s2b_synth_write_m5(const char* dir, uint64_t seed, int lo, int hi) {

@@ -92,6 +92,7 @@ int DitB200::check_errors() {
     if (dev_ < 0) return fail(ERR_STATE, "context not created");
     cudaSetDevice(dev_);
     if (int rc = shard_wait("check_errors", shard_ != nullptr)) return rc;
+    fold_status(stream_);       // flags of calls that launch no fold of their own
     return take_status(stream_, "an earlier stream-ordered call");
 }
 

@@ -161,6 +161,8 @@ public:
     int set_graph_last_layer(bool on);
 
     int precision() const { return prec_; }
+    int device() const { return dev_; }
+    void count_launches(int n) { launches_ += n; }
     uint64_t device_bytes() const;
     int last_launches() const { return last_launches_; }
     std::string err;

@@ -1,0 +1,289 @@
+// k_fp8_linear.cu -- y = sum_b xs[b, m] ws[n / 128, b] (xq . wq over block b) + bias
+// on the tcgen05 tensor cores (kind::f8f6f4, e4m3 codes), blocks of 128 along K.
+//
+// The scales change with every block of K, so a block's products cannot stay
+// in the accumulator: each block's fp32 sum (4 MMAs of 32 codes) goes to one
+// of two TMEM slots, and the epilogue warps read it and add scale * sum to
+// fp32 registers while the tensor core works on the next block.  Scales are
+// any fp32 values; sums and scale products are fp32, rounded once to y's type.
+#include "kcommon.cuh"
+#include "ops.h"
+#include "sm100.cuh"
+#include <atomic>
+#include <cuda.h>
+
+namespace s2b {
+
+// encoder of tensor maps over bytes (k_gemm_tc.cu)
+bool make_tmap_u8(CUtensorMap* m, const void* base, int rows, int cols, int ld, int box_rows);
+int gemm_tc_flag_ptr(int** p);
+
+namespace {
+
+constexpr int KB = 128;                  // K elements of a block (and bytes of a swizzled row)
+
+struct LinParams {
+    const float *xs, *ws, *bias;
+    void* y;
+    int M, N, nkb, ldy, y_type;
+    int* flag;                           // the GEMM class's device error flag
+};
+
+// Bounded wait; on expiry raises the CTA's abort flag and the device flag.
+__device__ __forceinline__ bool wait_flag(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* flag) {
+    for (uint32_t i = 0; i < sm100::WAIT_LIMIT; i++) {
+        if (sm100::mbar_try_wait(bar, parity)) return true;
+        if ((i & 1023) == 1023 && *abort_flag) return false;
+    }
+    *abort_flag = 1;
+    atomicExch(flag, 1);
+    return false;
+}
+
+__device__ __forceinline__ void store_y(void* y, int t, size_t i, float v) {
+    if (t == S2B_PREC_FP32) ((float*)y)[i] = v;
+    else if (t == S2B_PREC_FP16) ((f16*)y)[i] = __float2half_rn(v);
+    else ((bf16*)y)[i] = __float2bfloat16_rn(v);
+}
+
+// ---------------------------------------------------------------- few rows
+// Weights as the MMA's 128-row operand and BT tokens as its N: one token
+// fills 1/16 of an MMA instead of 1/128.  A cluster of `split` CTAs divides K
+// and joins its sums through shared memory in rank order (no atomics, no
+// workspace), so that few tiles still stream the weights from every SM.
+template <int BT> struct NarrowCfg {
+    static constexpr int W_BYTES = 128 * KB, X_BYTES = BT * KB, STAGE = W_BYTES + X_BYTES;
+    static constexpr int STAGES = BT == 64 ? 4 : 5;
+    static constexpr int COLS = BT == 16 ? 32 : 2 * BT;          // TMEM: two slots of BT columns
+    static constexpr int SMEM = STAGES * STAGE + 1024 + 256 + 4 * 2 * BT * 4;
+    static_assert(128 * BT * 4 <= STAGES * STAGE, "the joined sums reuse the stages");
+};
+template <int STAGES> struct NarrowCtl {
+    uint64_t full[STAGES], done[STAGES], tempty[2];
+    uint32_t tmem_slot;
+    int abort;
+};
+
+template <int BT>
+__global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant__ CUtensorMap mw,
+                                                           const __grid_constant__ CUtensorMap mx,
+                                                           const __grid_constant__ LinParams P, int split) {
+    using C = NarrowCfg<BT>;
+    constexpr int ST = C::STAGES;
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    NarrowCtl<ST>* ctl = reinterpret_cast<NarrowCtl<ST>*>(smem + ST * C::STAGE);
+    float* sc = reinterpret_cast<float*>(smem + ST * C::STAGE + 256);    // [4 warps][2][BT]
+    static_assert(sizeof(NarrowCtl<ST>) <= 256, "control block");
+    volatile int* abort_flag = &ctl->abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = split > 1 ? (int)sm100::cluster_ctarank() : 0;
+    const int tile = blockIdx.x / split;
+    const int ntn = (P.N + 127) / 128;
+    const int nb = tile % ntn, n0 = nb * 128, m0 = tile / ntn * BT;
+    const int kb0 = (int)((long)P.nkb * rank / split), kb1 = (int)((long)P.nkb * (rank + 1) / split);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < ST; s++) { sm100::mbar_init(&ctl->full[s], 1); sm100::mbar_init(&ctl->done[s], 1); }
+        sm100::mbar_init(&ctl->tempty[0], 4);
+        sm100::mbar_init(&ctl->tempty[1], 4);
+        ctl->abort = 0;
+        sm100::fence_barrier_init();
+        sm100::tma_prefetch_desc(&mw);
+        sm100::tma_prefetch_desc(&mx);
+    }
+    if (warp == 1) {
+        sm100::tmem_alloc(&ctl->tmem_slot, C::COLS);
+        sm100::tmem_relinquish();
+    }
+    sm100::tc_fence_before();
+    __syncthreads();
+    sm100::tc_fence_after();
+    const uint32_t tmem = ctl->tmem_slot;
+    float acc[BT];
+    #pragma unroll
+    for (int c = 0; c < BT; c++) acc[c] = 0.f;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 0;
+            long issued = 0;
+            for (int kb = kb0; kb < kb1; kb++) {
+                if (!wait_flag(&ctl->done[s], ph ^ 1, abort_flag, P.flag)) break;
+                uint8_t* st = smem + s * C::STAGE;
+                sm100::mbar_arrive_expect_tx(&ctl->full[s], C::STAGE);
+                sm100::tma_load_2d(st, &mw, &ctl->full[s], kb * KB, n0);
+                sm100::tma_load_2d(st + C::W_BYTES, &mx, &ctl->full[s], kb * KB, m0);
+                issued++;
+                if (++s == ST) { s = 0; ph ^= 1; }
+            }
+            // every load has landed before shared memory is used otherwise
+            for (long i = 1; i <= ST && i <= issued; i++) {
+                const long k = issued - i;
+                for (uint32_t w = 0; w < sm100::WAIT_LIMIT && !sm100::mbar_try_wait(&ctl->full[k % ST], (k / ST) & 1); w++) {}
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = sm100::idesc_e4m3_f32(128, BT);
+            int s = 0;
+            uint32_t ph = 0;
+            for (int kb = kb0; kb < kb1; kb++) {
+                const int i = kb - kb0, slot = i & 1;
+                if (!wait_flag(&ctl->tempty[slot], ((i >> 1) & 1) ^ 1, abort_flag, P.flag)) break;
+                if (!wait_flag(&ctl->full[s], ph, abort_flag, P.flag)) break;
+                sm100::tc_fence_after();
+                const uint8_t* st = smem + s * C::STAGE;
+                #pragma unroll
+                for (int k = 0; k < 4; k++)
+                    sm100::mma_f8(tmem + slot * BT, sm100::desc_kmajor_sw128(st, k * 32),
+                                  sm100::desc_kmajor_sw128(st + C::W_BYTES, k * 32), idesc, k != 0);
+                sm100::mma_commit(&ctl->done[s]);
+                if (++s == ST) { s = 0; ph ^= 1; }
+            }
+        }
+    } else {
+        const int q = warp & 3;
+        float* my = sc + (warp - 2) * 2 * BT;
+        const float* wrow = P.ws + (size_t)nb * P.nkb;
+        // scale products of a block: lane l holds tokens l and l + 32
+        auto fetch = [&](int kb, float v[2]) {
+            v[0] = v[1] = 0.f;
+            if (kb >= kb1) return;
+            const float w = __ldg(wrow + kb);
+            #pragma unroll
+            for (int j = 0; j < (BT + 31) / 32; j++) {
+                const int c = lane + 32 * j;
+                if (c < BT && m0 + c < P.M) v[j] = w * __ldg(P.xs + (size_t)kb * P.M + m0 + c);
+            }
+        };
+        float v[2], vn[2];
+        fetch(kb0, v);
+        int s = 0;
+        uint32_t ph = 0;
+        for (int kb = kb0; kb < kb1; kb++) {
+            const int slot = (kb - kb0) & 1;
+            float* sb = my + slot * BT;
+            #pragma unroll
+            for (int j = 0; j < (BT + 31) / 32; j++)
+                if (lane + 32 * j < BT) sb[lane + 32 * j] = v[j];
+            fetch(kb + 1, vn);
+            __syncwarp();
+            if (!__all_sync(0xffffffffu, wait_flag(&ctl->done[s], ph, abort_flag, P.flag))) break;
+            sm100::tc_fence_after();
+            #pragma unroll
+            for (int c0 = 0; c0 < BT; c0 += 16) {
+                float d[16];
+                sm100::tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + slot * BT + c0, d);
+                #pragma unroll
+                for (int c = 0; c < 16; c += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(sb + c0 + c);
+                    acc[c0 + c] = fmaf(d[c], f.x, acc[c0 + c]);
+                    acc[c0 + c + 1] = fmaf(d[c + 1], f.y, acc[c0 + c + 1]);
+                    acc[c0 + c + 2] = fmaf(d[c + 2], f.z, acc[c0 + c + 2]);
+                    acc[c0 + c + 3] = fmaf(d[c + 3], f.w, acc[c0 + c + 3]);
+                }
+            }
+            sm100::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&ctl->tempty[slot]);
+            v[0] = vn[0]; v[1] = vn[1];
+            if (++s == ST) { s = 0; ph ^= 1; }
+        }
+    }
+    __syncwarp();
+    __syncthreads();                     // every MMA and load of this CTA is done: the stages are free
+    const bool epi = warp >= 2;
+    const int nl = (warp & 3) * 32 + lane, n = n0 + nl;
+    if (split == 1) {
+        if (epi && n < P.N) {
+            const float b = P.bias ? __ldg(P.bias + n) : 0.f;
+            #pragma unroll
+            for (int c = 0; c < BT; c++)
+                if (m0 + c < P.M) store_y(P.y, P.y_type, (size_t)(m0 + c) * P.ldy + n, acc[c] + b);
+        }
+    } else {
+        float* red = reinterpret_cast<float*>(smem);             // [BT][128]
+        if (epi) {
+            #pragma unroll
+            for (int c = 0; c < BT; c++) red[c * 128 + nl] = acc[c];
+        }
+        sm100::cluster_sync();
+        if (epi && n < P.N) {
+            const float b = P.bias ? __ldg(P.bias + n) : 0.f;
+            for (int c = rank; c < BT; c += split) {
+                if (m0 + c >= P.M) break;
+                float t = 0.f;
+                for (int r = 0; r < split; r++) t += sm100::ld_cluster_f32(sm100::map_to_rank(red + c * 128 + nl, r));
+                store_y(P.y, P.y_type, (size_t)(m0 + c) * P.ldy + n, t + b);
+            }
+        }
+        sm100::cluster_sync();           // no CTA leaves while another reads its sums
+    }
+    if (warp == 1) {
+        sm100::tc_fence_after();
+        sm100::tmem_dealloc(tmem, C::COLS);
+    }
+}
+
+// Device address of the GEMM class's error flag, looked up once a device.
+int* device_flag() {
+    static std::atomic<int*> at[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return nullptr;
+    int* p = at[dev].load(std::memory_order_relaxed);
+    if (!p) {
+        if (gemm_tc_flag_ptr(&p)) return nullptr;
+        at[dev].store(p, std::memory_order_relaxed);
+    }
+    return p;
+}
+
+template <int BT>
+int launch_narrow(const Fp8LinearArgs& a, const LinParams& P, cudaStream_t s) {
+    using C = NarrowCfg<BT>;
+    CUtensorMap mw, mx;
+    if (!make_tmap_u8(&mw, a.wq, a.N, a.K, a.ldw, 128) || !make_tmap_u8(&mx, a.xq, a.M, a.K, a.ldx, BT)) return -1;
+    const long tiles = ((a.N + 127L) / 128) * ((a.M + BT - 1L) / BT);
+    // ranks along K: as many as two CTAs an SM hold, each with two blocks or more
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= 2L * op_sms() && P.nkb >= 4 * split) split *= 2;
+    if (tiles * split > 2147483647L) return -1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * split));
+    cfg.blockDim = dim3(192);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = split; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, k_fp8_linear_narrow<BT>, mw, mx, P, split) != cudaSuccess) return -1;
+    return 1;
+}
+
+}  // namespace
+
+int op_launch(const Fp8LinearArgs& a, cudaStream_t s) {
+    LinParams P;
+    P.xs = a.xs; P.ws = a.ws; P.bias = a.bias; P.y = a.y;
+    P.M = a.M; P.N = a.N; P.nkb = (int)((a.K + KB - 1L) / KB); P.ldy = a.ldy; P.y_type = a.y_type;
+    P.flag = device_flag();
+    if (!P.flag) return -1;
+    if (a.M <= 16) return launch_narrow<16>(a, P, s);
+    if (a.M <= 32) return launch_narrow<32>(a, P, s);
+    return launch_narrow<64>(a, P, s);
+}
+
+int fp8_linear_init_device() {
+    const void* f[3] = {(const void*)k_fp8_linear_narrow<16>, (const void*)k_fp8_linear_narrow<32>,
+                        (const void*)k_fp8_linear_narrow<64>};
+    const int b[3] = {NarrowCfg<16>::SMEM, NarrowCfg<32>::SMEM, NarrowCfg<64>::SMEM};
+    for (int i = 0; i < 3; i++)
+        if (cudaError_t e = cudaFuncSetAttribute(f[i], cudaFuncAttributeMaxDynamicSharedMemorySize, b[i])) return (int)e;
+    return 0;
+}
+
+}  // namespace s2b

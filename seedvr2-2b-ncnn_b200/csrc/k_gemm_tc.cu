@@ -925,6 +925,20 @@ bool make_tmap_bf16(CUtensorMap* m, const void* base, int rows, int cols, int ld
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Bytes [rows][cols] with row pitch ld; boxes of box_rows x 128 bytes (one
+// 128-byte swizzle row), zero fill: the 8-bit Linear's operand tiles.
+bool make_tmap_u8(CUtensorMap* m, const void* base, int rows, int cols, int ld, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // fp32 [rows][cols] (row stride ld elements), 32 x 32 boxes, 128-B swizzle:
 // the residual boxes of the gate/residual epilogue.
 static bool make_tmap_resid(CUtensorMap* m, const float* base, int rows, int cols, int ld) {
@@ -943,11 +957,13 @@ bool gemm_tc_supported(int M, int N, int K, int lda, int ldw) {
     return M > 0 && N > 0 && K > 0 && N % 32 == 0 && lda % 8 == 0 && ldw % 8 == 0 && encode_fn() != nullptr;
 }
 
-static int num_sms() {
+int op_sms() {
     int dev = 0;
     cudaGetDevice(&dev);
     return (dev < 64 && g_num_sms[dev] > 0) ? g_num_sms[dev] : 148;
 }
+
+static int num_sms() { return op_sms(); }
 
 static bool gemm_args_ok(const void* A, int lda, const void* W, int ldw, int M, int N, int K, const GemmEpi& e) {
     if (!gemm_tc_supported(M, N, K, lda, ldw)) return false;
@@ -1121,6 +1137,7 @@ int gemm_tc_flag_ptr(int** p) { return (int)cudaGetSymbolAddress((void**)p, g_tc
 
 int awa_init_device();
 int awa_tc_init_device();
+int fp8_linear_init_device();
 
 int kernels_init_device() {
     int dev = 0;
@@ -1145,6 +1162,7 @@ int kernels_init_device() {
         if (e != cudaSuccess) return (int)e;
     }
     if (int rc = awa_tc_init_device()) return rc;
+    if (int rc = fp8_linear_init_device()) return rc;
     return awa_init_device();
 }
 

@@ -26,6 +26,7 @@ LIB_PATH = os.path.join(_PKG, "lib", "libs2b.so")
 
 _F32P = ctypes.POINTER(ctypes.c_float)
 _I32P = ctypes.POINTER(ctypes.c_int)
+_L3 = ctypes.c_long * 3
 
 
 class S2BError(RuntimeError):
@@ -44,6 +45,23 @@ class s2b_win(ctypes.Structure):
                 ("st", _I32P), ("en", _I32P), ("sh", _I32P), ("eh", _I32P), ("sw", _I32P), ("ew", _I32P),
                 ("vid_freq", _F32P), ("n_vid_freq", ctypes.c_long),
                 ("txt_freq", _F32P), ("n_txt_freq", ctypes.c_long)]
+
+
+ROPE_MAX_PAIRS = 128
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+ACT_NONE, ACT_SILU = 0, 1
+
+
+class s2b_rope_config(ctypes.Structure):
+    _fields_ = [("layout", ctypes.c_int), ("axes", ctypes.c_int), ("axis_dim", ctypes.c_int * 3),
+                ("theta", ctypes.c_double), ("scaling", ctypes.c_int), ("factor", ctypes.c_double),
+                ("original_length", ctypes.c_double), ("beta_fast", ctypes.c_double), ("beta_slow", ctypes.c_double)]
+
+
+class s2b_rope(ctypes.Structure):
+    _fields_ = [("pairs", ctypes.c_int), ("half", ctypes.c_int), ("axes", ctypes.c_int), ("amplitude", ctypes.c_float),
+                ("turns", ctypes.c_uint64 * ROPE_MAX_PAIRS), ("axis", ctypes.c_uint8 * ROPE_MAX_PAIRS)]
 
 
 _lib = None
@@ -97,6 +115,14 @@ def lib() -> ctypes.CDLL:
         "s2b_forward_profile": [vp, _F32P, ip, _F32P, ip, ctypes.c_float, ctypes.POINTER(ctypes.c_double),
                                 ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double), _I32P],
         "s2b_linear_bf16_dev": [vp, vp, ip, ip, vp, ip, vp, vp, vp],
+        "s2b_fp8_quant_dev": [vp, vp, ip, ip, ip, ip, ip, vp, ip, vp, vp],
+        "s2b_linear_fp8_dev": [vp, vp, ip, vp, ip, ip, vp, ip, vp, ip, vp, vp, ip, ip, vp],
+        "s2b_rope_plan": [ctypes.POINTER(s2b_rope_config), ctypes.POINTER(s2b_rope)],
+        "s2b_rope_dev": [vp, ctypes.POINTER(s2b_rope), vp, ip, ip, ip, ip, ip, ctypes.POINTER(ctypes.c_long), vp,
+                         ctypes.c_long, ip, vp, ctypes.POINTER(ctypes.c_long), ip, vp],
+        "s2b_groupnorm_workspace": [ip, ip, ip, ip, ctypes.POINTER(ctypes.c_size_t)],
+        "s2b_groupnorm_dev": [vp, vp, ip, ip, ip, ip, ip, ip, vp, vp, ctypes.c_float, ip, vp, ip, ip, vp,
+                              ctypes.c_size_t, vp],
         "s2b_synth_write_m5": [ctypes.c_char_p, u64, ip, ip],
         "s2b_synth_vid_grid": [_F32P, ip, ip, ip, u64],
         "s2b_synth_txt": [_F32P, ip, u64],
@@ -335,6 +361,29 @@ def unpatchify_latent(sr: np.ndarray, T: int, H: int, W: int) -> np.ndarray:
     return out
 
 
+# ---------------------------------------------------------------- operators beside the DiT (host side)
+def rope_plan(axis_dims, layout: str = "interleaved", theta: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+              original_length: float = 0.0, beta_fast: float = 32.0, beta_slow: float = 1.0) -> s2b_rope:
+    """Rotary frequencies (s2b_rope_plan) of 1 to 3 axes; rope_plan([42, 42, 42]) is the DiT's own."""
+    if not 1 <= len(axis_dims) <= 3:
+        raise ValueError("axis_dims needs 1 to 3 entries")
+    if layout not in ROPE_LAYOUTS or scaling not in ROPE_SCALINGS:
+        raise ValueError(f"layout is one of {tuple(ROPE_LAYOUTS)}, scaling one of {tuple(ROPE_SCALINGS)}")
+    dims = (ctypes.c_int * 3)(*axis_dims)
+    cfg = s2b_rope_config(ROPE_LAYOUTS[layout], len(axis_dims), dims, theta, ROPE_SCALINGS[scaling], factor,
+                          original_length, beta_fast, beta_slow)
+    plan = s2b_rope()
+    _check(None, lib().s2b_rope_plan(ctypes.byref(cfg), ctypes.byref(plan)))
+    return plan
+
+
+def groupnorm_workspace(batch: int, rows: int, channels: int, groups: int) -> int:
+    """Bytes of device workspace that groupnorm_dev wants for these sizes."""
+    n = ctypes.c_size_t()
+    _check(None, lib().s2b_groupnorm_workspace(batch, rows, channels, groups, ctypes.byref(n)))
+    return n.value
+
+
 # ---------------------------------------------------------------- engine
 class DitB200:
     """The reference DitVk method set (src/dit_vk.h:24-121) on one B200."""
@@ -406,6 +455,31 @@ class DitB200:
     def linear_bf16_dev(self, d_x: int, M: int, K: int, d_w: int, N: int, d_bias, d_y: int, stream: int):
         """y = x W^T (+ bias) on device bf16 buffers (pointers as ints), enqueued on `stream`."""
         self._c(lib().s2b_linear_bf16_dev(self._ctx, d_x, M, K, d_w, N, d_bias, d_y, stream))
+
+    # ---- operators beside the DiT (device pointers as ints, types PREC_*, enqueued on `stream`)
+    def fp8_quant_dev(self, d_x: int, x_type: int, rows: int, cols: int, ldx: int, block_rows: int, d_q: int, ldq: int,
+                      d_scale: int, stream: int):
+        """e4m3 codes and scales of x in blocks of 128 columns x 1 or 128 rows (s2b_fp8_quant_dev)."""
+        self._c(lib().s2b_fp8_quant_dev(self._ctx, d_x, x_type, rows, cols, ldx, block_rows, d_q, ldq, d_scale, stream))
+
+    def linear_fp8_dev(self, d_xq: int, ldx: int, d_xs: int, M: int, K: int, d_wq: int, ldw: int, d_ws: int, N: int,
+                       d_bias, d_y: int, y_type: int, ldy: int, stream: int):
+        """y = (xq . xs) (wq . ws)^T (+ bias) on 8-bit codes (s2b_linear_fp8_dev)."""
+        self._c(lib().s2b_linear_fp8_dev(self._ctx, d_xq, ldx, d_xs, M, K, d_wq, ldw, d_ws, N, d_bias, d_y, y_type,
+                                         ldy, stream))
+
+    def rope_dev(self, plan: s2b_rope, d_x: int, x_type: int, batch: int, tokens: int, heads: int, head_dim: int,
+                 x_strides, d_pos, pos_batch_stride: int, pos0: int, d_y: int, y_strides, inverse: bool, stream: int):
+        """Rotary positions (s2b_rope_dev); strides are (batch, token, head) in elements."""
+        self._c(lib().s2b_rope_dev(self._ctx, plan, d_x, x_type, batch, tokens, heads, head_dim, _L3(*x_strides),
+                                   d_pos, pos_batch_stride, pos0, d_y, _L3(*y_strides), bool(inverse), stream))
+
+    def groupnorm_dev(self, d_x: int, x_type: int, batch: int, rows: int, channels: int, ldx: int, groups: int, d_gamma,
+                      d_beta, eps: float, act: int, d_y: int, y_type: int, ldy: int, d_work, work_bytes: int,
+                      stream: int):
+        """GroupNorm (+ SiLU) over channel-last rows (s2b_groupnorm_dev)."""
+        self._c(lib().s2b_groupnorm_dev(self._ctx, d_x, x_type, batch, rows, channels, ldx, groups, d_gamma, d_beta,
+                                        eps, act, d_y, y_type, ldy, d_work, work_bytes, stream))
 
     def forward_grid(self, vid_grid, txt, TXT, timestep=1000.0):
         T, H, W, _ = vid_grid.shape
