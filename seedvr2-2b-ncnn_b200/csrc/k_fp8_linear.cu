@@ -445,25 +445,30 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
                     const long k = issued - i;
                     for (uint32_t w = 0; w < sm100::WAIT_LIMIT && !sm100::mbar_try_wait(&ctl->full[k % PSTAGES], (k / PSTAGES) & 1); w++) {}
                 }
-        } else if (warp == 1 && lane == 0 && rank == 0) {
+        } else if (warp == 1 && rank == 0) {
             constexpr uint32_t idesc = sm100::idesc_e4m3_f32(PBM, PBN);
+            const uint64_t da = sm100::desc_kmajor_sw128(smem, 0), db = sm100::desc_kmajor_sw128(smem + P_TILE, 0);
+            const long blocks = (long)((T.total - pair + npairs - 1) / npairs) * P.nkb;
             int s = 0;
-            uint32_t ph = 0, it = 0;
-            bool ok = true;
-            for (int tile = pair; tile < T.total && ok; tile += npairs)
-                for (int kb = 0; kb < P.nkb; kb++, it++) {
-                    const uint32_t slot = it & 1;
-                    if (!wait_flag(&ctl->tempty[slot], ((it >> 1) & 1) ^ 1, abort_flag, P.flag) ||
-                        !wait_flag(&ctl->full[s], ph, abort_flag, P.flag)) { ok = false; break; }
-                    sm100::tc_fence_after();
-                    const uint8_t* st = smem + s * P_STAGE;
+            uint32_t ph = 0, use = 0;
+            const bool lead = sm100::elect_one();
+            for (long blk = 0; blk < blocks; blk++) {
+                const uint32_t slot = (uint32_t)(blk & 1);
+                bool ok = __all_sync(0xffffffffu, wait_flag(&ctl->full[s], ph, abort_flag, P.flag)) &&
+                          __all_sync(0xffffffffu, wait_flag(&ctl->tempty[slot], use ^ 1, abort_flag, P.flag));
+                if (!ok) break;
+                const uint64_t oa = da + (uint64_t)(s * P_STAGE >> 4), ob = db + (uint64_t)(s * P_STAGE >> 4);
+                sm100::tc_fence_after();
+                if (lead) {
                     #pragma unroll
                     for (int k = 0; k < 4; k++)
-                        sm100::mma_f8_pair(tmem + slot * PBN, sm100::desc_kmajor_sw128(st, k * 32),
-                                           sm100::desc_kmajor_sw128(st + P_TILE, k * 32), idesc, k != 0);
+                        sm100::mma_f8_pair(tmem + slot * PBN, oa + 2 * k, ob + 2 * k, idesc, k != 0);
                     sm100::mma_commit_pair_mc(&ctl->done[s], 0x3);
-                    if (++s == PSTAGES) { s = 0; ph ^= 1; }
                 }
+                __syncwarp();
+                if (++s == PSTAGES) { s = 0; ph ^= 1; }
+                use ^= (uint32_t)blk & 1;
+            }
         }
     } else {
         sm100::regs_grow<P_REGS_HIGH>();
