@@ -9,32 +9,34 @@
 // only rounding is the one to e4m3: the codes equal the definition's bit for
 // bit.  NaN and infinities become the code's NaN; they take no part in amax.
 //
-// Bound by HBM: e + 1 bytes per element.  Half a warp holds one 128-column
-// row segment, 8 elements a lane in one or two 16-byte loads; the maximum of
-// |x| is taken on the bit patterns (ordered like the values), two 16-bit
-// elements at a time.
+// Bound by HBM: e + 1 bytes per element.  A lane holds 32 bytes of a row, one
+// 256-bit load (16 elements of a 16-bit type, 8 of fp32), so 8 or 16 lanes hold
+// a block's row; the maximum of |x| is taken on the bit patterns (ordered like
+// the values), two 16-bit elements at a time.
 #include "kcommon.cuh"
 #include "ops.h"
 
 namespace s2b {
 namespace {
 
-template <typename T> struct Bits;      // patterns of 8 elements, as packed 32-bit words
+constexpr int WORDS = 8;               // 32-bit words a lane holds of a row
+
+template <typename T> struct Bits;      // bit patterns of a lane's elements, packed
 template <> struct Bits<float> {
-    static constexpr int WORDS = 8;
+    static constexpr int E = 8;         // elements a lane
     static constexpr uint32_t INF = 0x7F800000u;
     static __device__ __forceinline__ uint32_t mag(uint32_t w) { return w & 0x7FFFFFFFu; }
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { return max(a, b); }
     static __device__ __forceinline__ uint32_t fold(uint32_t w) { return w; }
     static __device__ __forceinline__ float value(uint32_t m) { return __uint_as_float(m); }
     static __device__ __forceinline__ uint32_t finite(uint32_t m) { return m < INF ? m : 0u; }
-    static __device__ __forceinline__ void floats(const uint32_t w[8], float v[8]) {
-        #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = __uint_as_float(w[i]);
+    // the two elements 2 i and 2 i + 1
+    static __device__ __forceinline__ float2 pair(const uint32_t w[WORDS], int i) {
+        return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
     }
 };
 template <typename H, uint32_t INF16> struct Bits16 {
-    static constexpr int WORDS = 4;
+    static constexpr int E = 16;
     static constexpr uint32_t INF = INF16;
     static __device__ __forceinline__ uint32_t mag(uint32_t w) { return w & 0x7FFF7FFFu; }
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
@@ -45,22 +47,14 @@ template <typename H, uint32_t INF16> struct Bits16 {
 };
 template <> struct Bits<bf16> : Bits16<bf16, 0x7F80u> {
     static __device__ __forceinline__ float value(uint32_t m) { return __uint_as_float(m << 16); }
-    static __device__ __forceinline__ void floats(const uint32_t w[4], float v[8]) {
-        #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
+    static __device__ __forceinline__ float2 pair(const uint32_t w[WORDS], int i) {
+        return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
     }
 };
 template <> struct Bits<f16> : Bits16<f16, 0x7C00u> {
     static __device__ __forceinline__ float value(uint32_t m) { return __half2float(__ushort_as_half((unsigned short)m)); }
-    static __device__ __forceinline__ void floats(const uint32_t w[4], float v[8]) {
-        #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            v[2 * i] = f.x; v[2 * i + 1] = f.y;
-        }
+    static __device__ __forceinline__ float2 pair(const uint32_t w[WORDS], int i) {
+        return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
     }
 };
 
@@ -80,22 +74,21 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return r;
 }
 
-// 8 elements from column c of a row (n of them inside it; the rest read 0).
+// A lane's elements from column c of a row (n of the row are left; what lies
+// past them reads 0).
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, long c, long n, uint32_t w[Bits<T>::WORDS]) {
-    #pragma unroll
-    for (int i = 0; i < Bits<T>::WORDS; i++) w[i] = 0;
-    if (n <= 0) return;
-    if (VEC && n >= 8) {
-        #pragma unroll
-        for (int i = 0; i < Bits<T>::WORDS / 4; i++) {
-            const uint4 t = __ldcs(reinterpret_cast<const uint4*>(row + c) + i);
-            w[4 * i] = t.x; w[4 * i + 1] = t.y; w[4 * i + 2] = t.z; w[4 * i + 3] = t.w;
-        }
+__device__ __forceinline__ void load_lane(const T* row, long c, long n, uint32_t w[WORDS]) {
+    constexpr int E = Bits<T>::E;
+    if (VEC && n >= E) {
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                     : "l"(row + c));
         return;
     }
     #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < WORDS; i++) w[i] = 0;
+    #pragma unroll
+    for (int i = 0; i < E; i++) {
         if (i >= n) break;
         if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(((const float*)row)[c + i]);
         else w[i / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(row)[c + i] << (16 * (i & 1));
@@ -103,79 +96,91 @@ __device__ __forceinline__ void load8(const T* row, long c, long n, uint32_t w[B
 }
 
 template <typename T>
-__device__ __forceinline__ uint32_t mag_max(const uint32_t w[Bits<T>::WORDS], bool finite_only) {
-    uint32_t m = 0;
+__device__ __forceinline__ uint32_t mag_max(const uint32_t w[WORDS]) {
+    uint32_t m = Bits<T>::mag(w[0]);
     #pragma unroll
-    for (int i = 0; i < Bits<T>::WORDS; i++) {
-        uint32_t a = Bits<T>::mag(w[i]);
-        if (finite_only) a = Bits<T>::finite(a);
-        m = Bits<T>::max2(m, a);
-    }
+    for (int i = 1; i < WORDS; i++) m = Bits<T>::max2(m, Bits<T>::mag(w[i]));
+    return Bits<T>::fold(m);
+}
+// The same over the finite elements (rare: out of line).
+template <typename T>
+__device__ __noinline__ uint32_t mag_max_finite(uint4 a, uint4 b) {
+    const uint32_t w[WORDS] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    uint32_t m = 0;
+    for (int i = 0; i < WORDS; i++) m = Bits<T>::max2(m, Bits<T>::finite(Bits<T>::mag(w[i])));
     return Bits<T>::fold(m);
 }
 
-// Codes of 8 elements times inv (a power of two), n of them inside the row.
-// `odd`: the block holds NaN or infinities, which become the code's NaN.
+// Codes of a lane's elements times inv (a power of two).  `odd`: the block
+// holds NaN or infinities, which become the code's NaN.
 template <typename T>
-__device__ __forceinline__ void store8(uint8_t* dst, const uint32_t w[Bits<T>::WORDS], float inv, long n, bool odd) {
-    float v[8];
-    Bits<T>::floats(w, v);
+__device__ __forceinline__ void store_lane(uint8_t* dst, const uint32_t w[WORDS], float inv, long n, bool odd) {
+    constexpr int E = Bits<T>::E;
+    uint32_t o[E / 4];
     #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        if (odd && !(fabsf(v[i]) < INFINITY)) v[i] = __uint_as_float(0x7FFFFFFFu);
-        else v[i] = __fmul_rn(v[i], inv);
+    for (int i = 0; i < E / 4; i++) {
+        float2 a = Bits<T>::pair(w, 2 * i), b = Bits<T>::pair(w, 2 * i + 1);
+        const float nan = __uint_as_float(0x7FFFFFFFu);
+        if (odd) {
+            if (!(fabsf(a.x) < INFINITY)) a.x = nan;
+            if (!(fabsf(a.y) < INFINITY)) a.y = nan;
+            if (!(fabsf(b.x) < INFINITY)) b.x = nan;
+            if (!(fabsf(b.y) < INFINITY)) b.y = nan;
+        }
+        o[i] = e4m3x2(__fmul_rn(a.x, inv), __fmul_rn(a.y, inv)) | e4m3x2(__fmul_rn(b.x, inv), __fmul_rn(b.y, inv)) << 16;
     }
-    const uint32_t lo = e4m3x2(v[0], v[1]) | e4m3x2(v[2], v[3]) << 16;
-    const uint32_t hi = e4m3x2(v[4], v[5]) | e4m3x2(v[6], v[7]) << 16;
-    if (n >= 8) {
-        *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+    if (n >= E) {
+        if constexpr (E == 16) *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+        else *reinterpret_cast<uint2*>(dst) = make_uint2(o[0], o[1]);
     } else {
         #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < n) dst[i] = (uint8_t)((i < 4 ? lo >> (8 * i) : hi >> (8 * (i - 4))) & 0xFFu);
+        for (int i = 0; i < E; i++)
+            if (i < n) dst[i] = (uint8_t)(o[i / 4] >> (8 * (i & 3)));
     }
 }
 
-// Rows: a CTA takes 32 rows x 512 columns; half-warp h rows h and h + 16,
-// four blocks each (eight 16-byte loads in flight a lane for 16-bit x).
-// Scales go out as 32 consecutive rows of one column block.
+// Largest of the LANES lanes that share a block's row.
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t m) {
+    #pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+
+// Rows: a CTA takes 32 rows x 512 columns, a lane group (8 lanes of a 16-bit
+// type, 16 of fp32) four blocks of one or two rows: four or eight 256-bit loads
+// in flight a lane.  Scales go out as 32 consecutive rows of one column block.
 constexpr int QR_ROWS = 32, QR_BLKS = 4;
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_fp8_quant_rows(const T* __restrict__ x, int rows, int cols, int ldx,
-                                                        uint8_t* __restrict__ q, int ldq, float* __restrict__ scale) {
+__global__ void __launch_bounds__(256, 3) k_fp8_quant_rows(const T* __restrict__ x, int rows, int cols, int ldx,
+                                                           uint8_t* __restrict__ q, int ldq, float* __restrict__ scale) {
+    constexpr int LANES = 128 / Bits<T>::E, GROUPS = 256 / LANES;
     __shared__ float ss[QR_BLKS][QR_ROWS];
-    const int hw = threadIdx.x >> 4, l = threadIdx.x & 15;
+    const int grp = threadIdx.x / LANES, l = threadIdx.x % LANES;
     const int kb = cols / 128 + (cols % 128 != 0), across = (kb + QR_BLKS - 1) / QR_BLKS;
     const long r0 = (long)(blockIdx.x / across) * QR_ROWS;
     const int b0 = blockIdx.x % across * QR_BLKS;
-    uint32_t w[2][QR_BLKS][Bits<T>::WORDS];
-    #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const long r = r0 + hw + 16 * i;
+    for (int i = grp; i < QR_ROWS; i += GROUPS) {
+        const long r = r0 + i;
+        if (r0 + i - grp >= rows) break;             // uniform: nothing left for any group
+        const long left = r < rows ? cols : 0;
+        uint32_t w[QR_BLKS][WORDS];
         #pragma unroll
         for (int j = 0; j < QR_BLKS; j++) {
-            const long c = (b0 + j) * 128L + l * 8;
-            load8<T, VEC>(x + (size_t)r * ldx, c, r < rows ? cols - c : 0, w[i][j]);
+            const long c = (b0 + j) * 128L + l * Bits<T>::E;
+            load_lane<T, VEC>(x + (size_t)r * ldx, c, left - c, w[j]);
         }
-    }
-    #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const long r = r0 + hw + 16 * i;
         #pragma unroll
         for (int j = 0; j < QR_BLKS; j++) {
-            const long c = (b0 + j) * 128L + l * 8;
-            uint32_t m = mag_max<T>(w[i][j], false);
-            #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const long c = (b0 + j) * 128L + l * Bits<T>::E;
+            uint32_t m = lanes_max<LANES>(mag_max<T>(w[j]));
             const bool odd = __any_sync(0xffffffffu, m >= Bits<T>::INF);
-            if (odd) {                               // rare: NaN or infinity in either half-warp's block
-                m = mag_max<T>(w[i][j], true);
-                #pragma unroll
-                for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            }
+            if (odd)                                 // rare: NaN or infinity in one of the warp's blocks
+                m = lanes_max<LANES>(mag_max_finite<T>(make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]),
+                                                       make_uint4(w[j][4], w[j][5], w[j][6], w[j][7])));
             const uint32_t e = scale_exp(Bits<T>::value(m));
-            if (r < rows && c < cols) store8<T>(q + (size_t)r * ldq + c, w[i][j], pow2_biased(254 - e), cols - c, odd);
-            if (l == 0) ss[j][hw + 16 * i] = pow2_biased(e);
+            if (c < left) store_lane<T>(q + (size_t)r * ldq + c, w[j], pow2_biased(254 - e), left - c, odd);
+            if (l == 0) ss[j][i] = pow2_biased(e);
         }
     }
     __syncthreads();
@@ -185,34 +190,34 @@ __global__ void __launch_bounds__(256) k_fp8_quant_rows(const T* __restrict__ x,
     }
 }
 
-// Weights: a CTA takes one 128 x 128 block, eight rows a half-warp, held in
-// registers between the maximum and the codes.
+// Weights: a CTA takes one 128 x 128 block, held in registers between the
+// maximum and the codes.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_fp8_quant_blocks(const T* __restrict__ x, int rows, int cols, int ldx,
-                                                          uint8_t* __restrict__ q, int ldq, float* __restrict__ scale) {
+__global__ void __launch_bounds__(256, 2) k_fp8_quant_blocks(const T* __restrict__ x, int rows, int cols, int ldx,
+                                                             uint8_t* __restrict__ q, int ldq, float* __restrict__ scale) {
+    constexpr int LANES = 128 / Bits<T>::E, GROUPS = 256 / LANES, PER = 128 / GROUPS;     // rows a lane
     __shared__ uint32_t sm[8], sf[8];
-    const int hw = threadIdx.x >> 4, l = threadIdx.x & 15, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int grp = threadIdx.x / LANES, l = threadIdx.x % LANES, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int kb = cols / 128 + (cols % 128 != 0);
-    const long c = blockIdx.x % kb * 128L + l * 8, rb = blockIdx.x / kb;
-    uint32_t w[8][Bits<T>::WORDS];
+    const long c = blockIdx.x % kb * 128L + l * Bits<T>::E, rb = blockIdx.x / kb;
+    uint32_t w[PER][WORDS];
     uint32_t m = 0, f = 0;
     #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const long r = rb * 128 + hw + 16 * i;
-        load8<T, VEC>(x + (size_t)r * ldx, c, r < rows ? cols - c : 0, w[i]);
+    for (int i = 0; i < PER; i++) {
+        const long r = rb * 128 + grp + GROUPS * i;
+        load_lane<T, VEC>(x + (size_t)r * ldx, c, r < rows ? cols - c : 0, w[i]);
     }
     #pragma unroll
-    for (int i = 0; i < 8; i++) m = max(m, mag_max<T>(w[i], false));
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int i = 0; i < PER; i++) m = max(m, mag_max<T>(w[i]));
+    m = lanes_max<32>(m);
     const bool warp_odd = m >= Bits<T>::INF;
     f = m;
     if (warp_odd) {                                  // rare, and the same for the whole warp
         f = 0;
         #pragma unroll
-        for (int i = 0; i < 8; i++) f = max(f, mag_max<T>(w[i], true));
-        #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) f = max(f, __shfl_xor_sync(0xffffffffu, f, o));
+        for (int i = 0; i < PER; i++)
+            f = max(f, mag_max_finite<T>(make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]), make_uint4(w[i][4], w[i][5], w[i][6], w[i][7])));
+        f = lanes_max<32>(f);
     }
     if (lane == 0) { sm[warp] = warp_odd; sf[warp] = f; }
     __syncthreads();
@@ -222,9 +227,9 @@ __global__ void __launch_bounds__(256) k_fp8_quant_blocks(const T* __restrict__ 
     const uint32_t e = scale_exp(Bits<T>::value(top));
     if (threadIdx.x == 0) scale[blockIdx.x] = pow2_biased(e);
     #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const long r = rb * 128 + hw + 16 * i;
-        if (r < rows && c < cols) store8<T>(q + (size_t)r * ldq + c, w[i], pow2_biased(254 - e), cols - c, any != 0);
+    for (int i = 0; i < PER; i++) {
+        const long r = rb * 128 + grp + GROUPS * i;
+        if (r < rows && c < cols) store_lane<T>(q + (size_t)r * ldq + c, w[i], pow2_biased(254 - e), cols - c, any != 0);
     }
 }
 
@@ -232,7 +237,8 @@ template <typename T>
 int launch(const Fp8QuantArgs& a, cudaStream_t s) {
     const T* x = (const T*)a.x;
     uint8_t* q = (uint8_t*)a.q;
-    const bool vec = ((uintptr_t)a.x & 15) == 0 && ((size_t)a.ldx * sizeof(T)) % 16 == 0;
+    // 256-bit loads where every row starts on 32 bytes, single elements elsewhere
+    const bool vec = ((uintptr_t)a.x & 31) == 0 && ((size_t)a.ldx * sizeof(T)) % 32 == 0;
     const long kb = (a.cols + 127L) / 128;
     if (a.block_rows == 1) {
         const long g = ((kb + QR_BLKS - 1) / QR_BLKS) * ((a.rows + QR_ROWS - 1L) / QR_ROWS);
