@@ -41,6 +41,19 @@ __device__ __forceinline__ bool wait_flag(uint64_t* bar, uint32_t parity, volati
     return false;
 }
 
+// The same for waits of thousands of cycles: the warp sleeps between polls and
+// leaves the issue slots of its scheduler to the warps that feed the tensor core.
+__device__ __forceinline__ bool wait_flag_idle(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* flag) {
+    for (uint32_t i = 0; i < (1u << 22); i++) {
+        if (sm100::mbar_try_wait(bar, parity)) return true;
+        if ((i & 255) == 255 && *abort_flag) return false;
+        __nanosleep(100);
+    }
+    *abort_flag = 1;
+    atomicExch(flag, 1);
+    return false;
+}
+
 __device__ __forceinline__ void store_y(void* y, int t, size_t i, float v) {
     if (t == S2B_PREC_FP32) ((float*)y)[i] = v;
     else if (t == S2B_PREC_FP16) ((f16*)y)[i] = __float2half_rn(v);
@@ -55,15 +68,46 @@ __device__ __forceinline__ void store_y(void* y, int t, size_t i, float v) {
 template <int BT> struct NarrowCfg {
     static constexpr int W_BYTES = 128 * KB, X_BYTES = BT * KB, STAGE = W_BYTES + X_BYTES;
     static constexpr int STAGES = BT == 64 ? 4 : 5;
-    static constexpr int COLS = BT == 16 ? 32 : 2 * BT;          // TMEM: two slots of BT columns
-    static constexpr int SMEM = STAGES * STAGE + 1024 + 256 + 4 * 2 * BT * 4;
+    // TMEM slots of BT columns: as many as 256 columns hold (two CTAs an SM).  A
+    // rank of a split K has fewer blocks than that, so its MMAs never wait for
+    // the epilogue.
+    static constexpr int COLS = 256, SLOTS = COLS / BT;
+    static constexpr int SMEM = STAGES * STAGE + 1024 + 512 + 4 * 2 * BT * 4;
     static_assert(128 * BT * 4 <= STAGES * STAGE, "the joined sums reuse the stages");
 };
-template <int STAGES> struct NarrowCtl {
-    uint64_t full[STAGES], done[STAGES], tempty[2];
+template <int STAGES, int SLOTS> struct NarrowCtl {
+    uint64_t full[STAGES], done[STAGES], tfull[SLOTS], tempty[SLOTS];
     uint32_t tmem_slot;
     int abort;
 };
+
+// Sums the ranks' column sums at red (stride 128 a token) in rank order and
+// writes this rank's tokens (rank, rank + SPLIT, ..) of weight row n.  All loads
+// of two tokens are in flight together.
+template <int BT, int SPLIT>
+__device__ __forceinline__ void join_ranks(const LinParams& P, float* red, int rank, int m0, int n) {
+    const float b = P.bias ? __ldg(P.bias + n) : 0.f;
+    uint32_t at[SPLIT];
+    #pragma unroll
+    for (int r = 0; r < SPLIT; r++) at[r] = sm100::map_to_rank(red, r);
+    #pragma unroll
+    for (int c0 = 0; c0 < BT; c0 += 2 * SPLIT) {
+        float v[2][SPLIT];
+        if (m0 + c0 + rank >= P.M) break;
+        #pragma unroll
+        for (int j = 0; j < 2; j++)
+            #pragma unroll
+            for (int r = 0; r < SPLIT; r++) v[j][r] = sm100::ld_cluster_f32(at[r] + (c0 + j * SPLIT + rank) * 512);
+        #pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int m = m0 + c0 + j * SPLIT + rank;
+            float t = v[j][0];
+            #pragma unroll
+            for (int r = 1; r < SPLIT; r++) t += v[j][r];
+            if (m < P.M) store_y(P.y, P.y_type, (size_t)m * P.ldy + n, t + b);
+        }
+    }
+}
 
 template <int BT>
 __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant__ CUtensorMap mw,
@@ -73,9 +117,10 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
     constexpr int ST = C::STAGES;
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    NarrowCtl<ST>* ctl = reinterpret_cast<NarrowCtl<ST>*>(smem + ST * C::STAGE);
-    float* sc = reinterpret_cast<float*>(smem + ST * C::STAGE + 256);    // [4 warps][2][BT]
-    static_assert(sizeof(NarrowCtl<ST>) <= 256, "control block");
+    typedef NarrowCtl<ST, C::SLOTS> Ctl;
+    Ctl* ctl = reinterpret_cast<Ctl*>(smem + ST * C::STAGE);
+    float* sc = reinterpret_cast<float*>(smem + ST * C::STAGE + 512);    // [4 warps][2][BT]
+    static_assert(sizeof(Ctl) <= 512, "control block");
     volatile int* abort_flag = &ctl->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = split > 1 ? (int)sm100::cluster_ctarank() : 0;
@@ -86,8 +131,7 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; s++) { sm100::mbar_init(&ctl->full[s], 1); sm100::mbar_init(&ctl->done[s], 1); }
-        sm100::mbar_init(&ctl->tempty[0], 4);
-        sm100::mbar_init(&ctl->tempty[1], 4);
+        for (int i = 0; i < C::SLOTS; i++) { sm100::mbar_init(&ctl->tfull[i], 1); sm100::mbar_init(&ctl->tempty[i], 4); }
         ctl->abort = 0;
         sm100::fence_barrier_init();
         sm100::tma_prefetch_desc(&mw);
@@ -131,8 +175,8 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
             int s = 0;
             uint32_t ph = 0;
             for (int kb = kb0; kb < kb1; kb++) {
-                const int i = kb - kb0, slot = i & 1;
-                if (!wait_flag(&ctl->tempty[slot], ((i >> 1) & 1) ^ 1, abort_flag, P.flag)) break;
+                const int i = kb - kb0, slot = i % C::SLOTS;
+                if (i >= C::SLOTS && !wait_flag(&ctl->tempty[slot], ((i / C::SLOTS) & 1) ^ 1, abort_flag, P.flag)) break;
                 if (!wait_flag(&ctl->full[s], ph, abort_flag, P.flag)) break;
                 sm100::tc_fence_after();
                 const uint8_t* st = smem + s * C::STAGE;
@@ -141,6 +185,7 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
                     sm100::mma_f8(tmem + slot * BT, sm100::desc_kmajor_sw128(st, k * 32),
                                   sm100::desc_kmajor_sw128(st + C::W_BYTES, k * 32), idesc, k != 0);
                 sm100::mma_commit(&ctl->done[s]);
+                sm100::mma_commit(&ctl->tfull[slot]);
                 if (++s == ST) { s = 0; ph ^= 1; }
             }
         }
@@ -161,17 +206,15 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
         };
         float v[2], vn[2];
         fetch(kb0, v);
-        int s = 0;
-        uint32_t ph = 0;
         for (int kb = kb0; kb < kb1; kb++) {
-            const int slot = (kb - kb0) & 1;
-            float* sb = my + slot * BT;
+            const int i = kb - kb0, slot = i % C::SLOTS;
+            float* sb = my + (i & 1) * BT;
             #pragma unroll
             for (int j = 0; j < (BT + 31) / 32; j++)
                 if (lane + 32 * j < BT) sb[lane + 32 * j] = v[j];
             fetch(kb + 1, vn);
             __syncwarp();
-            if (!__all_sync(0xffffffffu, wait_flag(&ctl->done[s], ph, abort_flag, P.flag))) break;
+            if (!__all_sync(0xffffffffu, wait_flag(&ctl->tfull[slot], (i / C::SLOTS) & 1, abort_flag, P.flag))) break;
             sm100::tc_fence_after();
             #pragma unroll
             for (int c0 = 0; c0 < BT; c0 += 16) {
@@ -190,7 +233,6 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(&ctl->tempty[slot]);
             v[0] = vn[0]; v[1] = vn[1];
-            if (++s == ST) { s = 0; ph ^= 1; }
         }
     }
     __syncwarp();
@@ -212,13 +254,9 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
         }
         sm100::cluster_sync();
         if (epi && n < P.N) {
-            const float b = P.bias ? __ldg(P.bias + n) : 0.f;
-            for (int c = rank; c < BT; c += split) {
-                if (m0 + c >= P.M) break;
-                float t = 0.f;
-                for (int r = 0; r < split; r++) t += sm100::ld_cluster_f32(sm100::map_to_rank(red + c * 128 + nl, r));
-                store_y(P.y, P.y_type, (size_t)(m0 + c) * P.ldy + n, t + b);
-            }
+            if (split == 2) join_ranks<BT, 2>(P, red + nl, rank, m0, n);
+            else if (split == 4) join_ranks<BT, 4>(P, red + nl, rank, m0, n);
+            else join_ranks<BT, 8>(P, red + nl, rank, m0, n);
         }
         sm100::cluster_sync();           // no CTA leaves while another reads its sums
     }
@@ -266,23 +304,48 @@ int launch_narrow(const Fp8LinearArgs& a, const LinParams& P, cudaStream_t s) {
 }
 
 // ---------------------------------------------------------------- many rows
-// Persistent CTA pairs (cta_group::2), 256 x 256 tiles: a CTA holds 128 rows
-// of A and 128 of B of every block of K, its 128 x 256 fp32 sums fill one of
-// the two TMEM slots.  Warp 0 loads, warp 1 of the even CTA issues the MMAs,
-// eight epilogue warps each own 32 rows x 128 columns -- one weight block, so
-// a thread's scale is one number a block -- and keep 128 sums in registers.
-// The MMAs of a block take 512 cycles of the tensor core; reading the sums
-// (256 columns a lane quadrant) and 64 packed FMAs a thread take fewer.
-constexpr int PBM = 256, PBN = 256, PSTAGES = 5, PTHREADS = 384;
-constexpr int P_TILE = 128 * KB, P_STAGE = 2 * P_TILE, P_BOX = 32 * 128;
-constexpr int P_SMEM = PSTAGES * P_STAGE + 8 * 2 * P_BOX + 1024 + 512;
-// Register shares: 168 a thread at launch; the epilogue's eight warps take 224
-// of the four others' 168 - 56.
-constexpr int P_REGS = 168, P_REGS_LOW = 56, P_REGS_HIGH = 224;
-static_assert(128 * P_REGS_LOW + 256 * P_REGS_HIGH <= PTHREADS * P_REGS, "register shares exceed the launch's");
+// Persistent CTA pairs (cta_group::2), tiles of 256 rows x BN columns: a CTA
+// holds 128 rows of A and BN / 2 of B of every block of K and gets 128 x BN
+// fp32 sums in one of two TMEM slots.  Each tile runs one of two ways:
+//
+//   scaled   every scale of the tile is a power of two (what the quantiser
+//            writes): the tensor core applies them (kind::mxf8f6f4, one E8M0
+//            byte a row and 32 codes; the four MMAs of a block use one byte)
+//            and sums the whole of K in a slot.  The epilogue of a tile runs
+//            beside the next tile's MMAs.
+//   general  any fp32 scales: a block's sum goes to a slot, the epilogue warps
+//            add scale * sum to registers while the next block runs.
+//
+// The general way is bound by the round trip MMA -> commit -> TMEM read ->
+// release -> MMA, about 2000 cycles for two blocks of 600 (5498 x 2560 x 13824:
+// 226 us); the scaled one by the tensor core.
+//
+// Warpgroup 0: warps 0 and 2 load by TMA, warp 1 (even CTA) issues the MMAs.
+// Warpgroup 1 looks at each tile's scales, a tile ahead or more, agrees with the
+// other CTA's on the way, and writes the scale bytes of four blocks at a
+// time to TMEM.  Warpgroups 2 and 3 are the epilogue: a warp owns 32 rows and
+// CH0 (the rest) chunks of 32 columns -- a chunk lies in one weight block.
+// Two consecutive blocks share one full barrier (a wait costs the MMA warp about
+// 200 cycles), each stage has its own done barrier (loads follow one by one).
+constexpr int PBM = 256, PSTAGES = 6, PBARS = PSTAGES / 2, PTHREADS = 512, RING = 4;
+// Register shares: 128 a thread at launch.
+constexpr int P_REGS = 128, P_REGS_0 = 48, P_REGS_1 = 80, P_REGS_EPI = 192;
+static_assert(P_REGS_0 + P_REGS_1 + 2 * P_REGS_EPI <= 4 * P_REGS, "register shares exceed the launch's");
 
-struct PairCtl {
-    uint64_t full[PSTAGES], done[PSTAGES], tempty[2];
+template <int BN> struct PairCfg8 {
+    static constexpr int CH = BN / 32, CH0 = (CH + 1) / 2;       // chunks of a tile, of warpgroup 2
+    static constexpr int A_TILE = 128 * KB, B_TILE = BN / 2 * KB, STAGE = A_TILE + B_TILE;
+    static constexpr int BOX = 4096;                             // a warp's staging: 2 chunks of 16-bit y, 1 of fp32
+    static constexpr int SMEM = PSTAGES * STAGE + 8 * BOX + 1024 + 1024;
+    static constexpr int SF = 2 * BN;                            // TMEM column of the scale bytes: RING x 16
+    static_assert(SF + RING * 16 <= 512 && BN % 32 == 0 && CH <= 8 && STAGE % 1024 == 0, "TMEM and tile layout");
+};
+
+struct alignas(16) PairCtl {
+    uint64_t full[PBARS], done[PSTAGES], tfull[2], tempty[2];
+    uint64_t sfull[RING], sempty[RING];          // scale bytes of four blocks
+    uint64_t mfull[RING], mempty[RING];          // the way a tile runs
+    uint4 odd[RING][2];                          // word q of CTA r: a scale that its warp q looked at is no power of two
     uint32_t tmem_slot;
     int abort;
 };
@@ -298,8 +361,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
-__device__ __forceinline__ float lo_f(uint64_t v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float hi_f(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
 
 // Two values in y's 16-bit type.
 __device__ __forceinline__ uint32_t half2_bits(float a, float b, int t) {
@@ -311,101 +372,85 @@ __device__ __forceinline__ uint32_t half2_bits(float a, float b, int t) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Writes 32 rows x 128 columns from (row0, col0): lane = row, acc its columns,
-// through this warp's two staging boxes of 32 rows x 128 bytes (128-byte
-// swizzle: conflict-free 16-byte stores).  Leaves its TMA stores in flight.
-__device__ __forceinline__ void pair_store(const LinParams& P, const PairTiles& T, const CUtensorMap* my, uint8_t* box, int row0,
-                                           int col0, uint64_t acc[64]) {
+// Lane = row: 32 columns of it into a staging box of 32 rows x 128 bytes (fp32)
+// or x 64 bytes (16-bit), swizzled so that the 16-byte stores hit all banks.
+// `bias` is lane l's: column l's.
+template <bool BIAS>
+__device__ __forceinline__ void stage_chunk(uint8_t* box, const uint32_t v[32], float bias, int type) {
     const int lane = threadIdx.x & 31;
-    if (lane == 0) sm100::bulk_wait_read_all();          // the boxes' previous stores
-    __syncwarp();
-    if (P.bias) {
-        float* b = reinterpret_cast<float*>(box);
+    auto at = [&](int i) { return BIAS ? __uint_as_float(v[i]) + __shfl_sync(0xffffffffu, bias, i) : __uint_as_float(v[i]); };
+    if (type == S2B_PREC_FP32) {
+        #pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float4 f = make_float4(at(4 * j), at(4 * j + 1), at(4 * j + 2), at(4 * j + 3));
+            *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) = f;
+        }
+    } else {
         #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int c = col0 + lane + 32 * j;
-            b[lane + 32 * j] = c < P.N ? __ldg(P.bias + c) : 0.f;
-        }
-        __syncwarp();
-        #pragma unroll
-        for (int j = 0; j < 32; j++) {
-            const float4 f = reinterpret_cast<const float4*>(b)[j];
-            acc[2 * j] = pack2(__float_as_uint(lo_f(acc[2 * j]) + f.x), __float_as_uint(hi_f(acc[2 * j]) + f.y));
-            acc[2 * j + 1] = pack2(__float_as_uint(lo_f(acc[2 * j + 1]) + f.z), __float_as_uint(hi_f(acc[2 * j + 1]) + f.w));
-        }
-        __syncwarp();
-    }
-    const bool wide = P.y_type == S2B_PREC_FP32;
-    const int per = wide ? 32 : 64;                      // columns of a box
-    #pragma unroll
-    for (int pass = 0; pass < 2; pass++) {
-        if (pass && !wide) break;
-        if (pass) {
-            if (lane == 0) sm100::bulk_wait_read_all();
-            __syncwarp();
-        }
-        #pragma unroll
-        for (int b = 0; b < 2; b++) {
-            #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                uint4 v;
-                if (wide) {
-                    const uint64_t *a = acc + pass * 32 + b * 16 + j * 2;
-                    v = make_uint4((uint32_t)a[0], (uint32_t)(a[0] >> 32), (uint32_t)a[1], (uint32_t)(a[1] >> 32));
-                } else {
-                    const uint64_t *a = acc + b * 32 + j * 4;
-                    v.x = half2_bits(lo_f(a[0]), hi_f(a[0]), P.y_type);
-                    v.y = half2_bits(lo_f(a[1]), hi_f(a[1]), P.y_type);
-                    v.z = half2_bits(lo_f(a[2]), hi_f(a[2]), P.y_type);
-                    v.w = half2_bits(lo_f(a[3]), hi_f(a[3]), P.y_type);
-                }
-                *reinterpret_cast<uint4*>(box + b * P_BOX + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
-            }
-        }
-        const int c0 = col0 + pass * 64;
-        if (T.tma_y) {
-            sm100::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                for (int b = 0; b < 2; b++)
-                    if (row0 < P.M && c0 + b * per < P.N) sm100::tma_store_2d(my, box + b * P_BOX, c0 + b * per, row0);
-                sm100::bulk_commit_group();
-            }
-        } else {
-            __syncwarp();
-            const int rows = min(32, P.M - row0), e = wide ? 4 : 2;
-            for (int r = 0; r < rows; r++)
-                for (int c = lane; c < 2 * per; c += 32) {
-                    if (c0 + c >= P.N) break;
-                    const int k = c % per * e;           // byte of the box's row
-                    const uint8_t* src = box + c / per * P_BOX + r * 128 + (((k >> 4) ^ (r & 7)) << 4) + (k & 15);
-                    const size_t at = (size_t)(row0 + r) * P.ldy + c0 + c;
-                    if (wide) ((uint32_t*)P.y)[at] = *reinterpret_cast<const uint32_t*>(src);
-                    else ((uint16_t*)P.y)[at] = *reinterpret_cast<const uint16_t*>(src);
-                }
-            __syncwarp();
+            uint4 u;
+            u.x = half2_bits(at(8 * j), at(8 * j + 1), type);
+            u.y = half2_bits(at(8 * j + 2), at(8 * j + 3), type);
+            u.z = half2_bits(at(8 * j + 4), at(8 * j + 5), type);
+            u.w = half2_bits(at(8 * j + 6), at(8 * j + 7), type);
+            *reinterpret_cast<uint4*>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = u;
         }
     }
 }
 
+// The warp's staged box of 32 columns from column c to y: one TMA store, or
+// element by element where y's rows start on no 16 bytes.
+__device__ __forceinline__ void flush_chunk(const LinParams& P, const PairTiles& T, const CUtensorMap* my, const uint8_t* box, int row0,
+                                            int c) {
+    const int lane = threadIdx.x & 31;
+    if (row0 >= P.M || c >= P.N) return;
+    if (T.tma_y) {
+        if (lane == 0) sm100::tma_store_2d(my, box, c, row0);
+        return;
+    }
+    const int rows = min(32, P.M - row0);
+    if (c + lane >= P.N) return;
+    for (int r = 0; r < rows; r++) {
+        const size_t at = (size_t)(row0 + r) * P.ldy + c + lane;
+        if (P.y_type == S2B_PREC_FP32)
+            ((uint32_t*)P.y)[at] = *reinterpret_cast<const uint32_t*>(box + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+        else
+            ((uint16_t*)P.y)[at] = *reinterpret_cast<const uint16_t*>(box + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+    }
+}
+
+// Positive normal powers of two are what an E8M0 byte (the exponent) can say.
+__device__ __forceinline__ bool no_power(float s) {
+    const uint32_t u = __float_as_uint(s);
+    return (u & 0x807FFFFFu) != 0 || u == 0 || u == 0x7F800000u;
+}
+
+template <int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PTHREADS, 1)
 k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw,
                   const __grid_constant__ CUtensorMap my, const __grid_constant__ LinParams P,
                   const __grid_constant__ PairTiles T) {
+    using C = PairCfg8<BN>;
     extern __shared__ uint8_t raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* boxes = smem + PSTAGES * P_STAGE;
-    PairCtl* ctl = reinterpret_cast<PairCtl*>(boxes + 8 * 2 * P_BOX);
-    static_assert(sizeof(PairCtl) <= 512, "control block");
+    uint8_t* boxes = smem + PSTAGES * C::STAGE;
+    PairCtl* ctl = reinterpret_cast<PairCtl*>(boxes + 8 * C::BOX);
+    static_assert(sizeof(PairCtl) <= 1024, "control block");
     volatile int* abort_flag = &ctl->abort;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2, q = warp & 3;
     const uint32_t rank = sm100::cluster_ctarank();
     const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < PSTAGES; s++) { sm100::mbar_init(&ctl->full[s], 1); sm100::mbar_init(&ctl->done[s], 1); }
-        sm100::mbar_init(&ctl->tempty[0], 16);
-        sm100::mbar_init(&ctl->tempty[1], 16);
+        for (int s = 0; s < PBARS; s++) sm100::mbar_init(&ctl->full[s], 1);
+        for (int s = 0; s < PSTAGES; s++) sm100::mbar_init(&ctl->done[s], 1);
+        for (int i = 0; i < 2; i++) { sm100::mbar_init(&ctl->tfull[i], 1); sm100::mbar_init(&ctl->tempty[i], 16); }
+        for (int i = 0; i < RING; i++) {
+            sm100::mbar_init(&ctl->sfull[i], 8);         // warpgroup 1 of both CTAs
+            sm100::mbar_init(&ctl->sempty[i], 1);
+            sm100::mbar_init(&ctl->mfull[i], 8);         // the same
+            sm100::mbar_init(&ctl->mempty[i], 25);       // 12 reading warps of each CTA and the MMA warp
+        }
         ctl->abort = 0;
         sm100::fence_barrier_init();
         sm100::tma_prefetch_desc(&mx);
@@ -420,115 +465,303 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
     sm100::tc_fence_after();
     const uint32_t tmem = ctl->tmem_slot;
 
-    if (warp < 4) {
-        sm100::regs_shrink<P_REGS_LOW>();
-        if (warp == 0 && lane == 0) {
-            int s = 0;
+    // The way tile number ti of this pair runs, read by a whole warp: 1
+    // scaled, 0 general, -1 when the wait expired.
+    auto tile_way = [&](uint32_t ti) -> int {
+        const uint32_t e = ti % RING, par = (ti / RING) & 1;
+        bool ok = false;
+        for (uint32_t i = 0; i < (1u << 22) && !ok; i++) {
+            ok = sm100::mbar_try_wait_cluster(&ctl->mfull[e], par);
+            if (!ok && (i & 1023) == 1023 && *abort_flag) break;
+            if (!ok && wg != 0) __nanosleep(100);
+        }
+        if (!__all_sync(0xffffffffu, ok)) {
+            *abort_flag = 1;
+            if (lane == 0) atomicExch(P.flag, 1);
+            return -1;
+        }
+        const uint4 a = ctl->odd[e][0], b = ctl->odd[e][1];
+        const int way = !(a.x | a.y | a.z | a.w | b.x | b.y | b.z | b.w);
+        __syncwarp();
+        if (lane < 2) sm100::mbar_arrive_cluster_cta(sm100::map_to_rank(&ctl->mempty[e], lane));
+        return way;
+    };
+
+    if (wg == 0) {
+        sm100::regs_shrink<P_REGS_0>();
+        if (warp != 1 && warp != 3 && lane == 0) {
+            // warp 0 loads A's tiles, warp 2 B's
+            const bool isb = warp == 2;
+            const CUtensorMap* map = isb ? &mw : &mx;
+            int s = 0;                                   // stage
             uint32_t ph = 0;
-            long issued = 0;
+            long issued = 0;                             // full barriers begun
             bool ok = true;
             for (int tile = pair; tile < T.total && ok; tile += npairs) {
-                const int xr = tile % T.num_m * PBM + (int)rank * 128, wr = tile / T.num_m * PBN + (int)rank * 128;
+                const int r = isb ? tile / T.num_m * BN + (int)rank * (BN / 2) : tile % T.num_m * PBM + (int)rank * 128;
                 for (int kb = 0; kb < P.nkb; kb++) {
                     // both CTAs' MMAs on this stage are done
                     if (!wait_flag(&ctl->done[s], ph ^ 1, abort_flag, P.flag)) { ok = false; break; }
-                    if (rank == 0) sm100::mbar_arrive_expect_tx(&ctl->full[s], 2 * P_STAGE);
-                    const uint32_t fb = sm100::map_to_rank(&ctl->full[s], 0);
-                    sm100::tma_load_2d_pair(smem + s * P_STAGE, &mx, fb, kb * KB, xr);
-                    sm100::tma_load_2d_pair(smem + s * P_STAGE + P_TILE, &mw, fb, kb * KB, wr);
-                    issued++;
-                    if (++s == PSTAGES) { s = 0; ph ^= 1; }
+                    const bool first = (kb & 1) == 0;
+                    if (first && !isb) {
+                        if (rank == 0) sm100::mbar_arrive_expect_tx(&ctl->full[s >> 1], min(2, P.nkb - kb) * 2 * C::STAGE);
+                        issued++;
+                    }
+                    const uint32_t fb = sm100::map_to_rank(&ctl->full[s >> 1], 0);
+                    sm100::tma_load_2d_pair(smem + s * C::STAGE + (isb ? C::A_TILE : 0), map, fb, kb * KB, r);
+                    s++;
+                    if (kb == P.nkb - 1 && first) s++;   // an odd block's partner stage stays empty
+                    if (s >= PSTAGES) { s = 0; ph ^= 1; }
                 }
             }
-            if (rank == 0)               // every load of the pair has landed (bounded) before anyone leaves
-                for (long i = 1; i <= PSTAGES && i <= issued; i++) {
+            if (rank == 0 && !isb)       // every load of the pair has landed (bounded) before anyone leaves
+                for (long i = 1; i <= PBARS && i <= issued; i++) {
                     const long k = issued - i;
-                    for (uint32_t w = 0; w < sm100::WAIT_LIMIT && !sm100::mbar_try_wait(&ctl->full[k % PSTAGES], (k / PSTAGES) & 1); w++) {}
+                    for (uint32_t w = 0; w < sm100::WAIT_LIMIT && !sm100::mbar_try_wait(&ctl->full[k % PBARS], (k / PBARS) & 1); w++) {}
                 }
         } else if (warp == 1 && rank == 0) {
-            constexpr uint32_t idesc = sm100::idesc_e4m3_f32(PBM, PBN);
-            const uint64_t da = sm100::desc_kmajor_sw128(smem, 0), db = sm100::desc_kmajor_sw128(smem + P_TILE, 0);
-            const long blocks = (long)((T.total - pair + npairs - 1) / npairs) * P.nkb;
-            int s = 0;
-            uint32_t ph = 0, use = 0;
+            constexpr uint32_t idesc = sm100::idesc_e4m3_f32(PBM, BN);
+            const uint64_t da = sm100::desc_kmajor_sw128(smem, 0), db = sm100::desc_kmajor_sw128(smem + C::A_TILE, 0);
             const bool lead = sm100::elect_one();
-            for (long blk = 0; blk < blocks; blk++) {
-                const uint32_t slot = (uint32_t)(blk & 1);
-                bool ok = __all_sync(0xffffffffu, wait_flag(&ctl->full[s], ph, abort_flag, P.flag)) &&
-                          __all_sync(0xffffffffu, wait_flag(&ctl->tempty[slot], use ^ 1, abort_flag, P.flag));
-                if (!ok) break;
-                const uint64_t oa = da + (uint64_t)(s * P_STAGE >> 4), ob = db + (uint64_t)(s * P_STAGE >> 4);
-                sm100::tc_fence_after();
-                if (lead) {
-                    #pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        sm100::mma_f8_pair(tmem + slot * PBN, oa + 2 * k, ob + 2 * k, idesc, k != 0);
-                    sm100::mma_commit_pair_mc(&ctl->done[s], 0x3);
+            int s = 0;
+            uint32_t ph = 0, use = 0, grp = 0, ti = 0;     // stage, slot uses, groups of scale bytes, tiles
+            bool ok = true;
+            auto wait = [&](uint64_t* bar, uint32_t par) { return __all_sync(0xffffffffu, wait_flag(bar, par, abort_flag, P.flag)) != 0; };
+            for (int tile = pair; tile < T.total && ok; tile += npairs, ti++) {
+                const int way = tile_way(ti);
+                if (way < 0) break;
+                if (way) {
+                    const uint32_t slot = use & 1, d = tmem + slot * BN;
+                    if (!(ok = wait(&ctl->tempty[slot], ((use >> 1) & 1) ^ 1))) break;
+                    for (int kb0 = 0; kb0 < P.nkb && ok; kb0 += 4, grp++) {
+                        if (!(ok = wait(&ctl->sfull[grp % RING], (grp / RING) & 1))) break;
+                        const uint32_t sf = tmem + C::SF + grp % RING * 16;
+                        #pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int left = P.nkb - kb0 - 2 * h;        // blocks from here
+                            if (left <= 0) break;
+                            if (!(ok = wait(&ctl->full[s], ph))) break;
+                            sm100::tc_fence_after();
+                            if (lead) {
+                                #pragma unroll
+                                for (int b = 0; b < 2; b++) {
+                                    if (b >= left) break;
+                                    const uint64_t off = (uint64_t)((2 * s + b) * C::STAGE >> 4);    // descriptors count 16-byte units
+                                    #pragma unroll
+                                    for (int k = 0; k < 4; k++)
+                                        sm100::mma_mxf8_pair(d, da + off + 2 * k, db + off + 2 * k, sm100::idesc_mxe4m3(PBM, BN, 2 * h + b), sf,
+                                                             sf + 4, (kb0 | h | b | k) != 0);
+                                    sm100::mma_commit_pair_mc(&ctl->done[2 * s + b], 0x3);
+                                }
+                                if (left == 1) sm100::mma_commit_pair_mc(&ctl->done[2 * s + 1], 0x3);    // the empty partner
+                            }
+                            __syncwarp();
+                            if (++s == PBARS) { s = 0; ph ^= 1; }
+                        }
+                        if (ok && lead) sm100::mma_commit_pair_mc(&ctl->sempty[grp % RING], 0x3);
+                        __syncwarp();
+                    }
+                    if (ok && lead) sm100::mma_commit_pair_mc(&ctl->tfull[slot], 0x3);
+                    __syncwarp();
+                    use++;
+                } else {
+                    for (int kb = 0; kb < P.nkb; kb++, use++) {
+                        const uint32_t slot = use & 1, d = tmem + slot * BN;
+                        if (!(kb & 1) && !(ok = wait(&ctl->full[s], ph))) break;
+                        if (!(ok = wait(&ctl->tempty[slot], ((use >> 1) & 1) ^ 1))) break;
+                        sm100::tc_fence_after();
+                        const bool last = (kb & 1) || kb == P.nkb - 1;
+                        if (lead) {
+                            const uint64_t off = (uint64_t)((2 * s + (kb & 1)) * C::STAGE >> 4);
+                            #pragma unroll
+                            for (int k = 0; k < 4; k++) sm100::mma_f8_pair(d, da + off + 2 * k, db + off + 2 * k, idesc, k != 0);
+                            sm100::mma_commit_pair_mc(&ctl->done[2 * s + (kb & 1)], 0x3);
+                            if (last && !(kb & 1)) sm100::mma_commit_pair_mc(&ctl->done[2 * s + 1], 0x3);    // the empty partner
+                            sm100::mma_commit_pair_mc(&ctl->tfull[slot], 0x3);
+                        }
+                        __syncwarp();
+                        if (last && ++s == PBARS) { s = 0; ph ^= 1; }
+                    }
                 }
-                __syncwarp();
-                if (++s == PSTAGES) { s = 0; ph ^= 1; }
-                use ^= (uint32_t)blk & 1;
             }
         }
-    } else {
-        sm100::regs_grow<P_REGS_HIGH>();
-        const int q = warp & 3, half = (warp - 4) >> 2;
-        uint8_t* box = boxes + (warp - 4) * 2 * P_BOX;
-        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + half * 128;
-        const int nwb = (P.N + KB - 1) / KB;
-        // scales run two blocks ahead of their use, across tiles
-        int ft = pair, fk = 0;
-        const float *fx = nullptr, *fw = nullptr;
-        auto next_scale = [&](float& x, float& w) {
-            if (ft >= T.total) { x = w = 0.f; return; }
-            if (fk == 0) {
-                const int row = ft % T.num_m * PBM + (int)rank * 128 + q * 32 + lane, wb = ft / T.num_m * 2 + half;
-                fx = row < P.M ? P.xs + row : nullptr;
-                fw = wb < nwb ? P.ws + (size_t)wb * P.nkb : nullptr;
+    } else if (wg == 1) {
+        sm100::regs_shrink<P_REGS_1>();
+        // A look at every scale of this CTA's part of tile number ti, a quarter a
+        // warp, posted to both CTAs.
+        auto look = [&](int tile, uint32_t ti) {
+            const int row = tile % T.num_m * PBM + (int)rank * 128 + (threadIdx.x & 127), n0 = tile / T.num_m * BN;
+            const int wb0 = n0 / KB, words = ((min(n0 + BN, P.N) - 1) / KB - wb0 + 1) * P.nkb;
+            bool odd = false;
+            if (row < P.M) {
+                const float* p = P.xs + row;
+                #pragma unroll 10
+                for (int kb = 0; kb < P.nkb; kb++) odd |= no_power(__ldg(p + (size_t)kb * P.M));
             }
-            x = fx ? __ldg(fx + (size_t)fk * P.M) : 0.f;
-            w = fw ? __ldg(fw + fk) : 0.f;
-            if (++fk == P.nkb) { fk = 0; ft += npairs; }
+            for (int i = threadIdx.x & 127; i < words; i += 128) odd |= no_power(__ldg(P.ws + (size_t)wb0 * P.nkb + i));
+            const uint32_t any = __any_sync(0xffffffffu, odd), e = ti % RING;
+            if (lane == 0) {
+                // the entry's readers of RING tiles ago are done, in both CTAs
+                wait_flag_idle(&ctl->mempty[e], ((ti / RING) & 1) ^ 1, abort_flag, P.flag);
+                for (uint32_t r = 0; r < 2; r++) {
+                    sm100::st_cluster_u32(sm100::map_to_rank(reinterpret_cast<uint32_t*>(&ctl->odd[e][rank]) + q, r), any);
+                    sm100::mbar_arrive_cluster(sm100::map_to_rank(&ctl->mfull[e], r));
+                }
+            }
+            __syncwarp();
         };
-        float x0, w0, x1, w1;
-        next_scale(x0, w0);
-        next_scale(x1, w1);
-        int s = 0;
-        uint32_t ph = 0, it = 0;
-        bool ok = true;
-        for (int tile = pair; tile < T.total; tile += npairs) {
-            uint64_t acc[64];
-            #pragma unroll
-            for (int i = 0; i < 64; i++) acc[i] = 0;
-            for (int kb = 0; kb < P.nkb; kb++, it++) {
-                const uint32_t sb = __float_as_uint(x0 * w0);
-                const uint64_t ss = pack2(sb, sb);
-                x0 = x1; w0 = w1;
-                next_scale(x1, w1);
-                const uint32_t slot = it & 1;
-                if (!__all_sync(0xffffffffu, wait_flag(&ctl->done[s], ph, abort_flag, P.flag))) { ok = false; break; }
-                sm100::tc_fence_after();
-                const uint32_t ta = taddr + slot * PBN;
-                uint32_t d[2][32];
-                sm100::tmem_ld32_async(ta, d[0]);
+        uint32_t grp = 0, ti = 0;
+        look(pair, 0);
+        for (int tile = pair; tile < T.total; tile += npairs, ti++) {
+            // the next tile's verdict is there before its MMAs ask for it
+            if (tile + npairs < T.total) look(tile + npairs, ti + 1);
+            const int m0 = tile % T.num_m * PBM + (int)rank * 128, n0 = tile / T.num_m * BN;
+            const int wb0 = n0 / KB, wbs = (min(n0 + BN, P.N) - 1) / KB - wb0 + 1;
+            const int way = tile_way(ti);
+            if (way < 0) break;
+            if (!way) continue;
+            // The next group's scales are on their way while this one is
+            // written: held as loaded, packed only when their turn comes.
+            struct Raw { float a[4][4], w[3][4]; };
+            auto load = [&](int kb0) {
+                Raw v;
                 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    sm100::tmem_wait32(d[j & 1]);
-                    if (j < 3) {
-                        sm100::tmem_ld32_async(ta + 32 * (j + 1), d[(j + 1) & 1]);
-                    } else {             // the slot is read: both CTAs' warps give it back to the MMA thread
-                        sm100::tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) sm100::mbar_arrive_cluster_cta(sm100::map_to_rank(&ctl->tempty[slot], 0));
+                for (int b = 0; b < 4; b++) {
+                    const bool in = kb0 + b < P.nkb;
+                    #pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int row = m0 + 32 * j + lane;
+                        v.a[j][b] = in && row < P.M ? __ldg(P.xs + (size_t)(kb0 + b) * P.M + row) : 1.f;
                     }
                     #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        acc[16 * j + i] = fma2(pack2(d[j & 1][2 * i], d[j & 1][2 * i + 1]), ss, acc[16 * j + i]);
+                    for (int j = 0; j < 3; j++) v.w[j][b] = in && j < wbs ? __ldg(P.ws + (size_t)(wb0 + j) * P.nkb + kb0 + b) : 1.f;
                 }
-                if (++s == PSTAGES) { s = 0; ph ^= 1; }
+                return v;
+            };
+            // byte b of a word: the exponent of block kb0 + b
+            auto pack = [](const float f[4]) {
+                return __float_as_uint(f[0]) >> 23 | __float_as_uint(f[1]) >> 23 << 8 | __float_as_uint(f[2]) >> 23 << 16 |
+                       __float_as_uint(f[3]) >> 23 << 24;
+            };
+            bool ok = true;
+            Raw next = load(0);
+            for (int kb0 = 0; kb0 < P.nkb; kb0 += 4, grp++) {
+                uint32_t sa[4], w3[3], sb[8];
+                #pragma unroll
+                for (int j = 0; j < 4; j++) sa[j] = pack(next.a[j]);
+                #pragma unroll
+                for (int j = 0; j < 3; j++) w3[j] = pack(next.w[j]);
+                #pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    const int j = (n0 + 32 * c) / KB - wb0;
+                    sb[c] = j == 0 ? w3[0] : j == 1 ? w3[1] : w3[2];
+                }
+                if (kb0 + 4 < P.nkb) next = load(kb0 + 4);
+                ok = __all_sync(0xffffffffu, wait_flag_idle(&ctl->sempty[grp % RING], ((grp / RING) & 1) ^ 1, abort_flag, P.flag));
+                if (!ok) break;
+                sm100::tc_fence_after();
+                const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + C::SF + grp % RING * 16;
+                sm100::tmem_st4(at, sa);
+                sm100::tmem_st8(at + 4, sb);
+                sm100::tmem_wait_st();
+                sm100::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) sm100::mbar_arrive_cluster_cta(sm100::map_to_rank(&ctl->sfull[grp % RING], 0));
             }
             if (!ok) break;
-            pair_store(P, T, &my, box, tile % T.num_m * PBM + (int)rank * 128 + q * 32, tile / T.num_m * PBN + half * 128, acc);
+        }
+    } else {
+        sm100::regs_grow<P_REGS_EPI>();
+        const int side = wg - 2, c0 = side * C::CH0, nc = side ? C::CH - C::CH0 : C::CH0;      // this warp's chunks
+        uint8_t* box = boxes + (warp - 8) * C::BOX;
+        const int per_box = P.y_type == S2B_PREC_FP32 ? 4096 : 2048, group = P.y_type == S2B_PREC_FP32 ? 1 : 2;
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + c0 * 32;
+        uint32_t tempty[2];
+        tempty[0] = sm100::map_to_rank(&ctl->tempty[0], 0);
+        tempty[1] = sm100::map_to_rank(&ctl->tempty[1], 0);
+        uint32_t use = 0, ti = 0;
+        bool ok = true;
+        for (int tile = pair; tile < T.total && ok; tile += npairs, ti++) {
+            const int row0 = tile % T.num_m * PBM + (int)rank * 128 + q * 32, n0 = tile / T.num_m * BN + c0 * 32;
+            const int way = tile_way(ti);
+            if (way < 0) break;
+            uint64_t acc[C::CH0][16];
+            if (!way) {
+                #pragma unroll
+                for (int c = 0; c < C::CH0; c++)
+                    #pragma unroll
+                    for (int i = 0; i < 16; i++) acc[c][i] = 0;
+                const float* px = row0 + lane < P.M ? P.xs + row0 + lane : nullptr;
+                const float* pw = P.ws + (size_t)(n0 / KB) * P.nkb;
+                const int nwb = (P.N + KB - 1) / KB;
+                // chunk c is in weight block n0 / KB + step(c)
+                auto step = [&](int c) { return (n0 % KB + 32 * c) / KB; };
+                float x1 = px ? __ldg(px) : 0.f;
+                for (int kb = 0; kb < P.nkb; kb++, use++) {
+                    const float x = x1;
+                    if (px && kb + 1 < P.nkb) x1 = __ldg(px + (size_t)(kb + 1) * P.M);
+                    float w[2];
+                    #pragma unroll
+                    for (int j = 0; j < 2; j++) w[j] = n0 / KB + j < nwb ? __ldg(pw + (size_t)j * P.nkb + kb) : 0.f;
+                    const uint32_t slot = use & 1;
+                    if (!__all_sync(0xffffffffu, wait_flag(&ctl->tfull[slot], (use >> 1) & 1, abort_flag, P.flag))) { ok = false; break; }
+                    sm100::tc_fence_after();
+                    #pragma unroll
+                    for (int c = 0; c < C::CH0; c++) {
+                        if (c >= nc) break;
+                        uint32_t d[32];
+                        sm100::tmem_ld32_async(taddr + slot * BN + 32 * c, d);
+                        sm100::tmem_wait32(d);
+                        if (c == nc - 1) {       // the slot is read: back to the MMA warp
+                            sm100::tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) sm100::mbar_arrive_cluster_cta(slot ? tempty[1] : tempty[0]);
+                        }
+                        const uint32_t sb = __float_as_uint(x * (step(c) ? w[1] : w[0]));
+                        const uint64_t ss = pack2(sb, sb);
+                        #pragma unroll
+                        for (int i = 0; i < 16; i++) acc[c][i] = fma2(pack2(d[2 * i], d[2 * i + 1]), ss, acc[c][i]);
+                    }
+                }
+                if (!ok) break;
+            } else if (!__all_sync(0xffffffffu, wait_flag_idle(&ctl->tfull[use & 1], (use >> 1) & 1, abort_flag, P.flag))) {
+                ok = false;
+                break;
+            }
+            sm100::tc_fence_after();
+            #pragma unroll
+            for (int c = 0; c < C::CH0; c++) {
+                if (c >= nc) break;
+                uint32_t d[32];
+                if (way) {
+                    sm100::tmem_ld32_async(taddr + (use & 1) * BN + 32 * c, d);
+                    sm100::tmem_wait32(d);
+                    if (c == nc - 1) {
+                        sm100::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) sm100::mbar_arrive_cluster_cta((use & 1) ? tempty[1] : tempty[0]);
+                    }
+                } else {
+                    #pragma unroll
+                    for (int i = 0; i < 16; i++) { d[2 * i] = (uint32_t)acc[c][i]; d[2 * i + 1] = (uint32_t)(acc[c][i] >> 32); }
+                }
+                const int col = n0 + 32 * c;
+                const float bias = P.bias && col + lane < P.N ? __ldg(P.bias + col + lane) : 0.f;
+                if (c % group == 0) {            // the staging's previous stores have been read
+                    if (lane == 0) sm100::bulk_wait_read_all();
+                    __syncwarp();
+                }
+                if (P.bias) stage_chunk<true>(box + c % group * per_box, d, bias, P.y_type);
+                else stage_chunk<false>(box + c % group * per_box, d, 0.f, P.y_type);
+                if (c % group == group - 1 || c == nc - 1) {
+                    if (T.tma_y) sm100::fence_proxy_async_smem();
+                    __syncwarp();
+                    for (int k = c - c % group; k <= c; k++) flush_chunk(P, T, &my, box + k % group * per_box, row0, n0 + 32 * k);
+                    if (T.tma_y && lane == 0) sm100::bulk_commit_group();
+                    __syncwarp();
+                }
+            }
+            if (way) use++;
         }
         if (lane == 0) sm100::bulk_wait_all();
     }
@@ -540,12 +773,13 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
     }
 }
 
+template <int BN>
 int launch_pair(const Fp8LinearArgs& a, const LinParams& P, cudaStream_t s) {
     CUtensorMap mx, mw, my;
-    if (!make_tmap_u8(&mx, a.xq, a.M, a.K, a.ldx, 128) || !make_tmap_u8(&mw, a.wq, a.N, a.K, a.ldw, 128)) return -1;
+    if (!make_tmap_u8(&mx, a.xq, a.M, a.K, a.ldx, 128) || !make_tmap_u8(&mw, a.wq, a.N, a.K, a.ldw, BN / 2)) return -1;
     PairTiles T;
     T.num_m = (a.M + PBM - 1) / PBM;
-    T.num_n = (a.N + PBN - 1) / PBN;
+    T.num_n = (a.N + BN - 1) / BN;
     const long tiles = (long)T.num_m * T.num_n;
     if (tiles > 2147483647L - 1024) return -1;
     T.total = (int)tiles;
@@ -558,7 +792,7 @@ int launch_pair(const Fp8LinearArgs& a, const LinParams& P, cudaStream_t s) {
     }
     int pairs = op_sms() / 2;
     if (T.total < pairs) pairs = T.total;
-    k_fp8_linear_pair<<<2 * pairs, PTHREADS, P_SMEM, s>>>(mx, mw, my, P, T);
+    k_fp8_linear_pair<BN><<<2 * pairs, PTHREADS, PairCfg8<BN>::SMEM, s>>>(mx, mw, my, P, T);
     return 1;
 }
 
@@ -570,8 +804,20 @@ int op_launch(const Fp8LinearArgs& a, cudaStream_t s) {
     P.M = a.M; P.N = a.N; P.nkb = (int)((a.K + KB - 1L) / KB); P.ldy = a.ldy; P.y_type = a.y_type;
     P.flag = device_flag();
     if (!P.flag) return -1;
-    static const int force = getenv("S2B_X") ? atoi(getenv("S2B_X")) : 0;
-    if (force == 1 || (!force && a.M > 256)) return launch_pair(a, P, s);
+    // The narrow kernel while its tiles are few enough for four ranks or more
+    // along K at two CTAs an SM; past that the pair kernel even where it leaves
+    // SMs idle (K 2560, N 2560: 192 rows 14.3 against 15.0 us, 256 rows 21.7
+    // against 15.1).
+    const long narrow = ((a.N + 127L) / 128) * ((a.M + 63L) / 64);
+    if (a.M > 64 && 4 * narrow > 2L * op_sms()) {
+        // The tile width with the cheaper waves: a 192-column tile takes 0.94 of
+        // a 224-column one's time.
+        const int pairs = op_sms() / 2;
+        const long tm = (a.M + PBM - 1L) / PBM;
+        const double w224 = (double)((tm * ((a.N + 223L) / 224) + pairs - 1) / pairs);
+        const double w192 = 0.94 * (double)((tm * ((a.N + 191L) / 192) + pairs - 1) / pairs);
+        return w192 < w224 ? launch_pair<192>(a, P, s) : launch_pair<224>(a, P, s);
+    }
     if (a.M <= 16) return launch_narrow<16>(a, P, s);
     if (a.M <= 32) return launch_narrow<32>(a, P, s);
     return launch_narrow<64>(a, P, s);
@@ -583,12 +829,17 @@ int fp8_linear_init_device() {
     const int b[3] = {NarrowCfg<16>::SMEM, NarrowCfg<32>::SMEM, NarrowCfg<64>::SMEM};
     for (int i = 0; i < 3; i++)
         if (cudaError_t e = cudaFuncSetAttribute(f[i], cudaFuncAttributeMaxDynamicSharedMemorySize, b[i])) return (int)e;
-    // the pair kernel's warpgroups exchange registers: they wait for ever if
+    // the pair kernels' warpgroups exchange registers: they wait for ever if
     // the kernel was compiled to fewer than their shares add up to
-    cudaFuncAttributes at;
-    if (cudaError_t e = cudaFuncGetAttributes(&at, (const void*)k_fp8_linear_pair)) return (int)e;
-    if (at.numRegs != P_REGS) return (int)cudaErrorInvalidKernelImage;
-    return (int)cudaFuncSetAttribute((const void*)k_fp8_linear_pair, cudaFuncAttributeMaxDynamicSharedMemorySize, P_SMEM);
+    const void* p[2] = {(const void*)k_fp8_linear_pair<224>, (const void*)k_fp8_linear_pair<192>};
+    const int pb[2] = {PairCfg8<224>::SMEM, PairCfg8<192>::SMEM};
+    for (int i = 0; i < 2; i++) {
+        cudaFuncAttributes at;
+        if (cudaError_t e = cudaFuncGetAttributes(&at, p[i])) return (int)e;
+        if (at.numRegs != P_REGS) return (int)cudaErrorInvalidKernelImage;
+        if (cudaError_t e = cudaFuncSetAttribute(p[i], cudaFuncAttributeMaxDynamicSharedMemorySize, pb[i])) return (int)e;
+    }
+    return 0;
 }
 
 }  // namespace s2b

@@ -941,18 +941,19 @@ bool make_tmap_u8(CUtensorMap* m, const void* base, int rows, int cols, int ld, 
 }
 
 // [rows][cols] of an S2B_PREC_* type (row pitch ld elements), boxes of 32 rows
-// x 128 bytes, 128-B swizzle: the 8-bit Linear's output boxes.
+// x 32 columns swizzled over their 128 (fp32) or 64 bytes: the 8-bit Linear's
+// output boxes.
 bool make_tmap_out(CUtensorMap* m, void* base, int type, int rows, int cols, int ld) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return false;
     const int e = type == PREC_FP32 ? 4 : 2;
     const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)ld * e};
-    const cuuint32_t box[2] = {(cuuint32_t)(128 / e), 32};
+    const cuuint32_t box[2] = {32, 32};
     const cuuint32_t estr[2] = {1, 1};
     const CUtensorMapDataType t = type == PREC_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                 : type == PREC_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    return fn(m, t, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    return fn(m, t, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, type == PREC_FP32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

@@ -245,6 +245,17 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float v[64]) {
     for (int i = 0; i < 64; i++) v[i] = __uint_as_float(r[i]);
 }
 
+// 4 / 8 consecutive columns of this warp's 32 lanes.
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t r[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t r[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
 // K-major operand tile written by TMA with 128-byte swizzle: rows of 128 B,
 // 8-row groups 1024 B apart.  `k_bytes` advances along K inside the 128-B
 // swizzle atom (the hardware applies the swizzle to the full address).
@@ -280,6 +291,22 @@ __device__ __forceinline__ uint32_t map_to_rank(const void* p, uint32_t rank) {
     uint32_t out;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(smem_u32(p)), "r"(rank));
     return out;
+}
+// Whether a phase is complete, acquiring what the other CTA wrote before it
+// arrived there.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P1;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P1, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, P1;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
 // A float of another CTA's shared memory (shared::cluster address).
 __device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
@@ -356,6 +383,24 @@ __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
         : "memory");
+}
+// kind::mxf8f6f4: the same with a power-of-two scale (E8M0 byte) for every row of
+// A and of B and 32 codes of K, read from TMEM at sfa / sfb: row r of A has its
+// byte in lane r % 32 (of each 32-lane quarter) of column r / 32, and the
+// instruction descriptor names which of the column's four bytes.
+__device__ __forceinline__ void mma_mxf8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
+                                              uint32_t sfb, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+        : "memory");
+}
+// Its instruction descriptor: e4m3 operands, E8M0 scales, byte `id` of the
+// scale columns of both operands.
+constexpr uint32_t idesc_mxe4m3(int M, int N, uint32_t id) {
+    return (id << 4) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27) | (id << 29);
 }
 // Instruction descriptor of kind::f8f6f4 with e4m3 operands (format 0) and
 // fp32 accumulators.
