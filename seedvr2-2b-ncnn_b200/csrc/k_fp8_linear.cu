@@ -72,7 +72,8 @@ template <int BT> struct NarrowCfg {
     // rank of a split K has fewer blocks than that, so its MMAs never wait for
     // the epilogue.
     static constexpr int COLS = 256, SLOTS = COLS / BT;
-    static constexpr int SMEM = STAGES * STAGE + 1024 + 512 + 4 * 2 * BT * 4;
+    static constexpr int G = SLOTS / 2 < 4 ? SLOTS / 2 : 4;      // blocks the epilogue takes at a time
+    static constexpr int SMEM = STAGES * STAGE + 1024 + 512 + 4 * G * BT * 4;
     static_assert(128 * BT * 4 <= STAGES * STAGE, "the joined sums reuse the stages");
 };
 template <int STAGES, int SLOTS> struct NarrowCtl {
@@ -81,31 +82,32 @@ template <int STAGES, int SLOTS> struct NarrowCtl {
     int abort;
 };
 
-// Sums the ranks' column sums at red (stride 128 a token) in rank order and
-// writes this rank's tokens (rank, rank + SPLIT, ..) of weight row n.  All loads
-// of two tokens are in flight together.
+// Sums the ranks' sums of weight row n in rank order and writes this rank's
+// tokens, four at a time: red is [BT / 4][128 weight rows][4 tokens].  Every load
+// from the other ranks is in flight before the first sum.
 template <int BT, int SPLIT>
-__device__ __forceinline__ void join_ranks(const LinParams& P, float* red, int rank, int m0, int n) {
+__device__ __forceinline__ void join_ranks(const LinParams& P, float4* red, int rank, int m0, int n) {
+    constexpr int G = (BT / 4 + SPLIT - 1) / SPLIT;      // groups of four tokens a rank
     const float b = P.bias ? __ldg(P.bias + n) : 0.f;
-    uint32_t at[SPLIT];
+    float4 v[G][SPLIT];
     #pragma unroll
-    for (int r = 0; r < SPLIT; r++) at[r] = sm100::map_to_rank(red, r);
+    for (int g = 0; g < G; g++) {
+        const int c4 = g * SPLIT + rank;
+        if (c4 * 4 >= BT || m0 + c4 * 4 >= P.M) break;
+        #pragma unroll
+        for (int r = 0; r < SPLIT; r++) v[g][r] = sm100::ld_cluster_f32x4(sm100::map_to_rank(red + c4 * 128, r));
+    }
     #pragma unroll
-    for (int c0 = 0; c0 < BT; c0 += 2 * SPLIT) {
-        float v[2][SPLIT];
-        if (m0 + c0 + rank >= P.M) break;
+    for (int g = 0; g < G; g++) {
+        const int m = m0 + (g * SPLIT + rank) * 4;
+        if ((g * SPLIT + rank) * 4 >= BT || m >= P.M) break;
+        float4 t = v[g][0];
         #pragma unroll
-        for (int j = 0; j < 2; j++)
-            #pragma unroll
-            for (int r = 0; r < SPLIT; r++) v[j][r] = sm100::ld_cluster_f32(at[r] + (c0 + j * SPLIT + rank) * 512);
+        for (int r = 1; r < SPLIT; r++) { t.x += v[g][r].x; t.y += v[g][r].y; t.z += v[g][r].z; t.w += v[g][r].w; }
+        const float o[4] = {t.x, t.y, t.z, t.w};
         #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int m = m0 + c0 + j * SPLIT + rank;
-            float t = v[j][0];
-            #pragma unroll
-            for (int r = 1; r < SPLIT; r++) t += v[j][r];
-            if (m < P.M) store_y(P.y, P.y_type, (size_t)m * P.ldy + n, t + b);
-        }
+        for (int i = 0; i < 4; i++)
+            if (m + i < P.M) store_y(P.y, P.y_type, (size_t)(m + i) * P.ldy + n, o[i] + b);
     }
 }
 
@@ -119,7 +121,7 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     typedef NarrowCtl<ST, C::SLOTS> Ctl;
     Ctl* ctl = reinterpret_cast<Ctl*>(smem + ST * C::STAGE);
-    float* sc = reinterpret_cast<float*>(smem + ST * C::STAGE + 512);    // [4 warps][2][BT]
+    float* sc = reinterpret_cast<float*>(smem + ST * C::STAGE + 512);    // [4 warps][G][BT]
     static_assert(sizeof(Ctl) <= 512, "control block");
     volatile int* abort_flag = &ctl->abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -129,13 +131,19 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
     const int nb = tile % ntn, n0 = nb * 128, m0 = tile / ntn * BT;
     const int kb0 = (int)((long)P.nkb * rank / split), kb1 = (int)((long)P.nkb * (rank + 1) / split);
 
+    auto load_block = [&](int kb, int s) {
+        uint8_t* st = smem + s * C::STAGE;
+        sm100::mbar_arrive_expect_tx(&ctl->full[s], C::STAGE);
+        sm100::tma_load_2d(st, &mw, &ctl->full[s], kb * KB, n0);
+        sm100::tma_load_2d(st + C::W_BYTES, &mx, &ctl->full[s], kb * KB, m0);
+    };
     if (threadIdx.x == 0) {
         for (int s = 0; s < ST; s++) { sm100::mbar_init(&ctl->full[s], 1); sm100::mbar_init(&ctl->done[s], 1); }
         for (int i = 0; i < C::SLOTS; i++) { sm100::mbar_init(&ctl->tfull[i], 1); sm100::mbar_init(&ctl->tempty[i], 4); }
         ctl->abort = 0;
         sm100::fence_barrier_init();
-        sm100::tma_prefetch_desc(&mw);
-        sm100::tma_prefetch_desc(&mx);
+        // the first loads are on their way while TMEM is allocated
+        for (int s = 0; s < ST && kb0 + s < kb1; s++) load_block(kb0 + s, s);
     }
     if (warp == 1) {
         sm100::tmem_alloc(&ctl->tmem_slot, C::COLS);
@@ -153,13 +161,10 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
         if (lane == 0) {
             int s = 0;
             uint32_t ph = 0;
-            long issued = 0;
-            for (int kb = kb0; kb < kb1; kb++) {
-                if (!wait_flag(&ctl->done[s], ph ^ 1, abort_flag, P.flag)) break;
-                uint8_t* st = smem + s * C::STAGE;
-                sm100::mbar_arrive_expect_tx(&ctl->full[s], C::STAGE);
-                sm100::tma_load_2d(st, &mw, &ctl->full[s], kb * KB, n0);
-                sm100::tma_load_2d(st + C::W_BYTES, &mx, &ctl->full[s], kb * KB, m0);
+            long issued = min(ST, kb1 - kb0);
+            for (int kb = kb0 + ST; kb < kb1; kb++) {
+                if (!wait_flag(&ctl->done[s], ph, abort_flag, P.flag)) break;
+                load_block(kb, s);
                 issued++;
                 if (++s == ST) { s = 0; ph ^= 1; }
             }
@@ -170,69 +175,83 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = sm100::idesc_e4m3_f32(128, BT);
-            int s = 0;
-            uint32_t ph = 0;
-            for (int kb = kb0; kb < kb1; kb++) {
-                const int i = kb - kb0, slot = i % C::SLOTS;
-                if (i >= C::SLOTS && !wait_flag(&ctl->tempty[slot], ((i / C::SLOTS) & 1) ^ 1, abort_flag, P.flag)) break;
-                if (!wait_flag(&ctl->full[s], ph, abort_flag, P.flag)) break;
-                sm100::tc_fence_after();
-                const uint8_t* st = smem + s * C::STAGE;
+        // the whole warp walks the loop and one elected lane issues: descriptors
+        // stay in uniform registers (a lane on its own took three times as long)
+        constexpr uint32_t idesc = sm100::idesc_e4m3_f32(128, BT);
+        const uint64_t dw = sm100::desc_kmajor_sw128(smem, 0), dx = sm100::desc_kmajor_sw128(smem + C::W_BYTES, 0);
+        const bool lead = sm100::elect_one();
+        auto wait = [&](uint64_t* bar, uint32_t par) { return __all_sync(0xffffffffu, wait_flag(bar, par, abort_flag, P.flag)) != 0; };
+        int s = 0;
+        uint32_t ph = 0;
+        for (int kb = kb0; kb < kb1; kb++) {
+            const int i = kb - kb0, slot = i % C::SLOTS;
+            if (i >= C::SLOTS && !wait(&ctl->tempty[slot], ((i / C::SLOTS) & 1) ^ 1)) break;
+            if (!wait(&ctl->full[s], ph)) break;
+            sm100::tc_fence_after();
+            if (lead) {
+                const uint64_t off = (uint64_t)(s * C::STAGE >> 4);      // descriptors count 16-byte units
                 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    sm100::mma_f8(tmem + slot * BT, sm100::desc_kmajor_sw128(st, k * 32),
-                                  sm100::desc_kmajor_sw128(st + C::W_BYTES, k * 32), idesc, k != 0);
-                sm100::mma_commit(&ctl->done[s]);
+                for (int k = 0; k < 4; k++) sm100::mma_f8(tmem + slot * BT, dw + off + 2 * k, dx + off + 2 * k, idesc, k != 0);
                 sm100::mma_commit(&ctl->tfull[slot]);
-                if (++s == ST) { s = 0; ph ^= 1; }
+                if (kb + ST < kb1) sm100::mma_commit(&ctl->done[s]);     // loaded again
             }
+            __syncwarp();
+            if (++s == ST) { s = 0; ph ^= 1; }
         }
     } else {
         const int q = warp & 3;
-        float* my = sc + (warp - 2) * 2 * BT;
+        constexpr int G = C::G, PER = (BT + 31) / 32;
+        float* my = sc + (warp - 2) * G * BT;
         const float* wrow = P.ws + (size_t)nb * P.nkb;
-        // scale products of a block: lane l holds tokens l and l + 32
-        auto fetch = [&](int kb, float v[2]) {
-            v[0] = v[1] = 0.f;
-            if (kb >= kb1) return;
-            const float w = __ldg(wrow + kb);
+        // Scales of the next G blocks as loaded: lane l holds tokens l and l + 32.
+        float w[G], x[G][PER];
+        auto fetch = [&](int kb, float& wv, float (&xv)[PER]) {
+            const bool in = kb < kb1;
+            wv = in ? __ldg(wrow + kb) : 0.f;
             #pragma unroll
-            for (int j = 0; j < (BT + 31) / 32; j++) {
+            for (int j = 0; j < PER; j++) {
                 const int c = lane + 32 * j;
-                if (c < BT && m0 + c < P.M) v[j] = w * __ldg(P.xs + (size_t)kb * P.M + m0 + c);
+                xv[j] = in && c < BT && m0 + c < P.M ? __ldg(P.xs + (size_t)kb * P.M + m0 + c) : 0.f;
             }
         };
-        float v[2], vn[2];
-        fetch(kb0, v);
-        for (int kb = kb0; kb < kb1; kb++) {
-            const int i = kb - kb0, slot = i % C::SLOTS;
-            float* sb = my + (i & 1) * BT;
+        #pragma unroll
+        for (int a = 0; a < G; a++) fetch(kb0 + a, w[a], x[a]);
+        // G blocks at a time, after the last one's MMAs (which end in order): one
+        // wait and one release instead of G, each a few hundred cycles
+        for (int kb = kb0; kb < kb1; kb += G) {
+            const int n = min(G, kb1 - kb), i0 = kb - kb0;
             #pragma unroll
-            for (int j = 0; j < (BT + 31) / 32; j++)
-                if (lane + 32 * j < BT) sb[lane + 32 * j] = v[j];
-            fetch(kb + 1, vn);
+            for (int a = 0; a < G; a++) {
+                #pragma unroll
+                for (int j = 0; j < PER; j++)
+                    if (lane + 32 * j < BT) my[a * BT + lane + 32 * j] = w[a] * x[a][j];
+                fetch(kb + G + a, w[a], x[a]);
+            }
             __syncwarp();
-            if (!__all_sync(0xffffffffu, wait_flag(&ctl->tfull[slot], (i / C::SLOTS) & 1, abort_flag, P.flag))) break;
+            const int last = i0 + n - 1;
+            if (!__all_sync(0xffffffffu, wait_flag(&ctl->tfull[last % C::SLOTS], (last / C::SLOTS) & 1, abort_flag, P.flag))) break;
             sm100::tc_fence_after();
             #pragma unroll
-            for (int c0 = 0; c0 < BT; c0 += 16) {
-                float d[16];
-                sm100::tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + slot * BT + c0, d);
+            for (int a = 0; a < G; a++) {
+                if (a >= n) break;
+                const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + (i0 + a) % C::SLOTS * BT;
                 #pragma unroll
-                for (int c = 0; c < 16; c += 4) {
-                    const float4 f = *reinterpret_cast<const float4*>(sb + c0 + c);
-                    acc[c0 + c] = fmaf(d[c], f.x, acc[c0 + c]);
-                    acc[c0 + c + 1] = fmaf(d[c + 1], f.y, acc[c0 + c + 1]);
-                    acc[c0 + c + 2] = fmaf(d[c + 2], f.z, acc[c0 + c + 2]);
-                    acc[c0 + c + 3] = fmaf(d[c + 3], f.w, acc[c0 + c + 3]);
+                for (int c0 = 0; c0 < BT; c0 += 16) {
+                    float d[16];
+                    sm100::tmem_ld16(ta + c0, d);
+                    #pragma unroll
+                    for (int c = 0; c < 16; c += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(my + a * BT + c0 + c);
+                        acc[c0 + c] = fmaf(d[c], f.x, acc[c0 + c]);
+                        acc[c0 + c + 1] = fmaf(d[c + 1], f.y, acc[c0 + c + 1]);
+                        acc[c0 + c + 2] = fmaf(d[c + 2], f.z, acc[c0 + c + 2]);
+                        acc[c0 + c + 3] = fmaf(d[c + 3], f.w, acc[c0 + c + 3]);
+                    }
                 }
             }
             sm100::tc_fence_before();
             __syncwarp();
-            if (lane == 0) sm100::mbar_arrive(&ctl->tempty[slot]);
-            v[0] = vn[0]; v[1] = vn[1];
+            if (lane < n) sm100::mbar_arrive(&ctl->tempty[(i0 + lane) % C::SLOTS]);
         }
     }
     __syncwarp();
@@ -247,16 +266,16 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
                 if (m0 + c < P.M) store_y(P.y, P.y_type, (size_t)(m0 + c) * P.ldy + n, acc[c] + b);
         }
     } else {
-        float* red = reinterpret_cast<float*>(smem);             // [BT][128]
+        float4* red = reinterpret_cast<float4*>(smem) + nl;      // [BT / 4][128] of four tokens
         if (epi) {
             #pragma unroll
-            for (int c = 0; c < BT; c++) red[c * 128 + nl] = acc[c];
+            for (int c = 0; c < BT; c += 4) red[c / 4 * 128] = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
         }
         sm100::cluster_sync();
         if (epi && n < P.N) {
-            if (split == 2) join_ranks<BT, 2>(P, red + nl, rank, m0, n);
-            else if (split == 4) join_ranks<BT, 4>(P, red + nl, rank, m0, n);
-            else join_ranks<BT, 8>(P, red + nl, rank, m0, n);
+            if (split == 2) join_ranks<BT, 2>(P, red, rank, m0, n);
+            else if (split == 4) join_ranks<BT, 4>(P, red, rank, m0, n);
+            else join_ranks<BT, 8>(P, red, rank, m0, n);
         }
         sm100::cluster_sync();           // no CTA leaves while another reads its sums
     }
