@@ -372,6 +372,42 @@ int s2b_groupnorm_dev(s2b_ctx* ctx, const void* d_x, int x_type, int batch, int 
                                           d_y, y_type, ldy, d_work, work_bytes}, stream);
 }
 
+int s2b_op_packed(const void* args) {
+    if (!args) return refuse(nullptr, S2B_ERR_ARG, "packed call: null argument");
+    int64_t a[24];
+    std::memcpy(a, args, sizeof a);
+    s2b_ctx* ctx = (s2b_ctx*)a[1];
+    // ints have to be ints: a 64-bit word that is none is refused, not cut
+    bool whole = true;
+    auto i = [&](int k) { whole = whole && a[k] == (int64_t)(int)a[k]; return (int)a[k]; };
+    auto p = [&](int k) { return (void*)a[k]; };
+    auto f = [&](int k) { return (const float*)a[k]; };
+    void* stream = p(2);
+    switch (a[0]) {
+        case S2B_OP_FP8_QUANT: {
+            const s2b::Fp8QuantArgs q{p(3), i(4), i(5), i(6), i(7), i(8), p(9), i(10), (float*)p(11)};
+            return whole ? run_op(ctx, q, stream) : refuse(ctx, S2B_ERR_ARG, "packed call: an int is out of range");
+        }
+        case S2B_OP_LINEAR_FP8: {
+            const s2b::Fp8LinearArgs q{p(3), i(4), f(5), i(6), i(7), p(8), i(9), f(10), i(11), f(12), p(13), i(14), i(15)};
+            return whole ? run_op(ctx, q, stream) : refuse(ctx, S2B_ERR_ARG, "packed call: an int is out of range");
+        }
+        case S2B_OP_ROPE: {
+            const s2b::RopeArgs q{(const s2b_rope*)p(3), p(4), i(5), i(6), i(7), i(8), i(9), {a[10], a[11], a[12]}, (const int*)p(13),
+                                  a[14], i(15), p(16), {a[17], a[18], a[19]}, i(20)};
+            return whole ? run_op(ctx, q, stream) : refuse(ctx, S2B_ERR_ARG, "packed call: an int is out of range");
+        }
+        case S2B_OP_GROUPNORM: {
+            double eps;
+            std::memcpy(&eps, &a[12], sizeof eps);
+            const s2b::GroupNormArgs q{p(3), i(4), i(5), i(6), i(7), i(8), i(9), f(10), f(11), (float)eps, i(13), p(14), i(15), i(16),
+                                       p(17), (size_t)a[18]};
+            return whole ? run_op(ctx, q, stream) : refuse(ctx, S2B_ERR_ARG, "packed call: an int is out of range");
+        }
+    }
+    return refuse(ctx, S2B_ERR_ARG, "packed call: unknown operator");
+}
+
 int s2b_synth_write_m5(const char* dir, uint64_t seed, int lo, int hi) {
     if (!dir) return S2B_ERR_ARG;
     std::string err;

@@ -7,6 +7,7 @@
 // fp32 registers while the tensor core works on the next block.  Scales are
 // any fp32 values; sums and scale products are fp32, rounded once to y's type.
 #include "kcommon.cuh"
+#include "launch.cuh"
 #include "ops.h"
 #include "sm100.cuh"
 #include <atomic>
@@ -142,6 +143,7 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
         for (int i = 0; i < C::SLOTS; i++) { sm100::mbar_init(&ctl->tfull[i], 1); sm100::mbar_init(&ctl->tempty[i], 4); }
         ctl->abort = 0;
         sm100::fence_barrier_init();
+        chain_wait();
         // the first loads are on their way while TMEM is allocated
         for (int s = 0; s < ST && kb0 + s < kb1; s++) load_block(kb0 + s, s);
     }
@@ -153,6 +155,8 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
     __syncthreads();
     sm100::tc_fence_after();
     const uint32_t tmem = ctl->tmem_slot;
+    chain_release();                     // not before this CTA has its TMEM: the next kernel's could take it first
+    chain_wait();
     float acc[BT];
     #pragma unroll
     for (int c = 0; c < BT; c++) acc[c] = 0.f;
@@ -308,18 +312,7 @@ int launch_narrow(const Fp8LinearArgs& a, const LinParams& P, cudaStream_t s) {
     int split = 1;
     while (split < 8 && tiles * split * 2 <= 2L * op_sms() && P.nkb >= 4 * split) split *= 2;
     if (tiles * split > 2147483647L) return -1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * split));
-    cfg.blockDim = dim3(192);
-    cfg.dynamicSmemBytes = C::SMEM;
-    cfg.stream = s;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = split; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, k_fp8_linear_narrow<BT>, mw, mx, P, split) != cudaSuccess) return -1;
-    return 1;
+    return launch_chained(k_fp8_linear_narrow<BT>, dim3((unsigned)(tiles * split)), 192, C::SMEM, split, s, mw, mx, P, split) ? 1 : -1;
 }
 
 // ---------------------------------------------------------------- many rows
@@ -483,6 +476,8 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
     sm100::cluster_sync();
     sm100::tc_fence_after();
     const uint32_t tmem = ctl->tmem_slot;
+    chain_release();                     // not before this CTA has its TMEM
+    chain_wait();
 
     // The way tile number ti of this pair runs, read by a whole warp: 1
     // scaled, 0 general, -1 when the wait expired.
@@ -811,8 +806,7 @@ int launch_pair(const Fp8LinearArgs& a, const LinParams& P, cudaStream_t s) {
     }
     int pairs = op_sms() / 2;
     if (T.total < pairs) pairs = T.total;
-    k_fp8_linear_pair<BN><<<2 * pairs, PTHREADS, PairCfg8<BN>::SMEM, s>>>(mx, mw, my, P, T);
-    return 1;
+    return launch_chained(k_fp8_linear_pair<BN>, dim3(2 * pairs), PTHREADS, PairCfg8<BN>::SMEM, 0, s, mx, mw, my, P, T) ? 1 : -1;
 }
 
 }  // namespace

@@ -14,6 +14,7 @@
 // a block's row; the maximum of |x| is taken on the bit patterns (ordered like
 // the values), two 16-bit elements at a time.
 #include "kcommon.cuh"
+#include "launch.cuh"
 #include "ops.h"
 
 namespace s2b {
@@ -156,6 +157,7 @@ __global__ void __launch_bounds__(256, 3) k_fp8_quant_rows(const T* __restrict__
                                                            uint8_t* __restrict__ q, int ldq, float* __restrict__ scale) {
     constexpr int LANES = 128 / Bits<T>::E, GROUPS = 256 / LANES;
     __shared__ float ss[QR_BLKS][QR_ROWS];
+    chain_begin();
     const int grp = threadIdx.x / LANES, l = threadIdx.x % LANES;
     const int kb = cols / 128 + (cols % 128 != 0), across = (kb + QR_BLKS - 1) / QR_BLKS;
     const long r0 = (long)(blockIdx.x / across) * QR_ROWS;
@@ -197,6 +199,7 @@ __global__ void __launch_bounds__(256, 2) k_fp8_quant_blocks(const T* __restrict
                                                              uint8_t* __restrict__ q, int ldq, float* __restrict__ scale) {
     constexpr int LANES = 128 / Bits<T>::E, GROUPS = 256 / LANES, PER = 128 / GROUPS;     // rows a lane
     __shared__ uint32_t sm[8], sf[8];
+    chain_begin();
     const int grp = threadIdx.x / LANES, l = threadIdx.x % LANES, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int kb = cols / 128 + (cols % 128 != 0);
     const long c = blockIdx.x % kb * 128L + l * Bits<T>::E, rb = blockIdx.x / kb;
@@ -243,15 +246,11 @@ int launch(const Fp8QuantArgs& a, cudaStream_t s) {
     if (a.block_rows == 1) {
         const long g = ((kb + QR_BLKS - 1) / QR_BLKS) * ((a.rows + QR_ROWS - 1L) / QR_ROWS);
         if (g > 2147483647L) return -1;
-        if (vec) k_fp8_quant_rows<T, true><<<(unsigned)g, 256, 0, s>>>(x, a.rows, a.cols, a.ldx, q, a.ldq, a.scale);
-        else k_fp8_quant_rows<T, false><<<(unsigned)g, 256, 0, s>>>(x, a.rows, a.cols, a.ldx, q, a.ldq, a.scale);
-        return 1;
+        return launch_chained(vec ? k_fp8_quant_rows<T, true> : k_fp8_quant_rows<T, false>, dim3((unsigned)g), 256, 0, 0, s, x, a.rows, a.cols, a.ldx, q, a.ldq, a.scale) ? 1 : -1;
     }
     const long g = kb * ((a.rows + 127L) / 128);
     if (g > 2147483647L) return -1;
-    if (vec) k_fp8_quant_blocks<T, true><<<(unsigned)g, 256, 0, s>>>(x, a.rows, a.cols, a.ldx, q, a.ldq, a.scale);
-    else k_fp8_quant_blocks<T, false><<<(unsigned)g, 256, 0, s>>>(x, a.rows, a.cols, a.ldx, q, a.ldq, a.scale);
-    return 1;
+    return launch_chained(vec ? k_fp8_quant_blocks<T, true> : k_fp8_quant_blocks<T, false>, dim3((unsigned)g), 256, 0, 0, s, x, a.rows, a.cols, a.ldx, q, a.ldq, a.scale) ? 1 : -1;
 }
 
 }  // namespace

@@ -20,9 +20,9 @@
 //   streamed  samples whose slabs exceed a cluster's registers: partial
 //             statistics of row chunks, their join per group, and the
 //             normalisation, which reads x again, last chunk first: what the
-//             statistics read last is still in L2.  The launches are chained
-//             (programmatic dependent launch).
+//             statistics read last is still in L2.
 #include "kcommon.cuh"
+#include "launch.cuh"
 #include "ops.h"
 #include "sm100.cuh"
 
@@ -90,9 +90,6 @@ __device__ __forceinline__ void join_groups(const float2* sm, int width, int lan
 // Vector columns a CTA covers and the rows it takes side by side.
 __host__ __device__ inline int tile_cols(int vecs) { return vecs < THREADS ? vecs : THREADS; }
 
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // SUB: channels of a vector that share a group, taken together (VEC, VEC / 2,
 // or 1 for groups that cut vectors otherwise).
 template <typename T, int VEC, int SUB>
@@ -100,7 +97,7 @@ __global__ void __launch_bounds__(THREADS, STATS_CTAS) k_gn_stats(const GnParams
     typedef Vec<T, VEC> V;
     constexpr int N = VEC / SUB, UNROLL = 8;
     __shared__ float2 sm[THREADS * N];
-    grid_release();                      // the join may be set up; it waits for this grid's end
+    chain_begin();
     const int vecs = P.C / VEC, tw = tile_cols(vecs), rp = THREADS / tw;
     const int tc = threadIdx.x % tw, tr = threadIdx.x / tw;
     const int vc = blockIdx.y * tw + tc;
@@ -169,12 +166,11 @@ __device__ __forceinline__ float4 finish(float ref, Moments m, float eps) {
 template <typename T>
 __global__ void __launch_bounds__(128) k_gn_join(const GnParams P) {
     __shared__ float4 sm[4];
-    grid_release();
+    chain_begin();
     const int g = blockIdx.x, b = blockIdx.y;
     const float ref = Cvt<T>::to_f(((const T*)P.x)[(size_t)b * P.rows * P.ldx + (size_t)g * P.cpg]);
     const int entries = P.chunks * P.tiles;
     const float4* part = P.part + (size_t)b * entries * P.G + g;
-    grid_wait();
     Moments a = {0.f, 0.f, 0.f};
     for (int e = threadIdx.x; e < entries; e += 4 * 128) {
         float4 v[4];
@@ -238,10 +234,10 @@ __global__ void __launch_bounds__(THREADS, APPLY_CTAS) k_gn_apply(const GnParams
     const int tc = threadIdx.x % tw, tr = threadIdx.x / tw;
     const int vc = blockIdx.y * tw + tc;
     const int b = gridDim.z - 1 - blockIdx.z;
+    chain_begin();
     if (tr >= rp || vc >= vecs) return;
     Affine<TX, TY, VEC, SUB> f;
     f.weights(P, vc * VEC);
-    grid_wait();                         // before the first read of what the join wrote
     #pragma unroll
     for (int i = 0; i < VEC / SUB; i++) f.stats(i, P.stat[(size_t)b * P.G + (vc * VEC + i * SUB) / P.cpg]);
     // tiles of U * rp rows, the CTAs side by side through the sample from its
@@ -279,6 +275,7 @@ __global__ void __launch_bounds__(THREADS, RV <= 4 ? 3 : 2) k_gn_chip(const GnPa
     __shared__ float4 mine[CHIP_GROUPS];         // this CTA's (n, mean - ref, M2) of the slab's groups
     __shared__ float4 stat[CHIP_GROUPS];
     __shared__ float sref[CHIP_GROUPS];
+    chain_begin();
     const int rank = P.split > 1 ? (int)sm100::cluster_ctarank() : 0;
     const int item = blockIdx.x / P.split, b = item / P.slabs, c0 = item % P.slabs * P.slab;
     const int vw = P.slab / VEC, rp = THREADS / vw, width = P.slab / SUB;
@@ -361,20 +358,6 @@ int chunk_rows(long batch, int rows, int per_sm, int round) {
     const long c = (rows + want - 1) / want;
     return (int)((c + round - 1) / round * round);
 }
-template <typename F, typename... A>
-bool launch_chained(F f, dim3 g, int threads, cudaStream_t s, const A&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = g;
-    cfg.blockDim = dim3(threads);
-    cfg.stream = s;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, f, args...) == cudaSuccess;
-}
-
 // The on-chip form's slab, cluster and vectors a thread; false when it does
 // not fit.  Slabs are the fewest whole groups that make rows of 64 bytes or
 // more (two sectors), clusters the smallest that hold a sample's slab and
@@ -405,17 +388,8 @@ bool plan_chip(const GroupNormArgs& a, int vec, int xe, GnParams& P, int& rv) {
 
 template <typename TX, typename TY, int VEC, int SUB>
 bool launch_chip(const GnParams& P, int batch, int rv, cudaStream_t s) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long)batch * P.slabs * P.split));
-    cfg.blockDim = dim3(THREADS);
-    cfg.stream = s;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = P.split; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    if (rv == 4) return cudaLaunchKernelEx(&cfg, k_gn_chip<TX, TY, VEC, SUB, 4>, P) == cudaSuccess;
-    return cudaLaunchKernelEx(&cfg, k_gn_chip<TX, TY, VEC, SUB, 16>, P) == cudaSuccess;
+    return launch_chained(rv == 4 ? k_gn_chip<TX, TY, VEC, SUB, 4> : k_gn_chip<TX, TY, VEC, SUB, 16>,
+                          dim3((unsigned)((long)batch * P.slabs * P.split)), THREADS, 0, P.split, s, P);
 }
 
 template <typename TX, typename TY, int VEC, int SUB>
@@ -432,9 +406,9 @@ int launch_v(const GroupNormArgs& a, GnParams& P, cudaStream_t s) {
     P.stat = (float4*)a.work;
     P.part = P.stat + (size_t)a.batch * P.G;
     const dim3 g(P.chunks, P.tiles, a.batch), ga((a.rows + achunk - 1) / achunk, P.tiles, a.batch);
-    k_gn_stats<TX, VEC, SUB><<<g, THREADS, 0, s>>>(P);
-    if (!launch_chained(k_gn_join<TX>, dim3(P.G, a.batch), 128, s, P)) return -1;
-    if (!launch_chained(k_gn_apply<TX, TY, VEC, SUB>, ga, THREADS, s, P)) return -1;
+    if (!launch_chained(k_gn_stats<TX, VEC, SUB>, g, THREADS, 0, 0, s, P)) return -1;
+    if (!launch_chained(k_gn_join<TX>, dim3(P.G, a.batch), 128, 0, 0, s, P)) return -1;
+    if (!launch_chained(k_gn_apply<TX, TY, VEC, SUB>, ga, THREADS, 0, 0, s, P)) return -1;
     return 3;
 }
 

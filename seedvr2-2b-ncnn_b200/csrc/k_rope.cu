@@ -14,6 +14,7 @@
 // order.  B200: 40 heads of 128 at 5440 tokens (111 MB) 25.7 us, 8 heads of 128
 // at 131042 tokens in fp32 (1.07 GB) 191 us, 5.6 TB/s.
 #include "kcommon.cuh"
+#include "launch.cuh"
 #include "ops.h"
 
 namespace s2b {
@@ -166,6 +167,7 @@ __global__ void __launch_bounds__(256, ROPE_CTAS) k_rope(const __grid_constant__
         S.axis[threadIdx.x] = P.p.axis[threadIdx.x];
     }
     __syncthreads();
+    chain_begin();
     unsigned at = blockIdx.x;
     const int chunk = at % P.chunks;
     at /= P.chunks;
@@ -186,9 +188,7 @@ int launch_hu(RopeParams& P, long ctas, cudaStream_t s) {
     P.chunks = P.heads / HU;
     const long g = ctas * P.chunks;
     if (g > 2147483647L) return -1;
-    if (P.p.half) k_rope<T, VEC, true, HU><<<(unsigned)g, 256, 0, s>>>(P);
-    else k_rope<T, VEC, false, HU><<<(unsigned)g, 256, 0, s>>>(P);
-    return 1;
+    return launch_chained(P.p.half ? k_rope<T, VEC, true, HU> : k_rope<T, VEC, false, HU>, dim3((unsigned)g), 256, 0, 0, s, P) ? 1 : -1;
 }
 
 template <typename T, int VEC>

@@ -1,0 +1,40 @@
+// launch.cuh -- launches of the operators beside the DiT, chained by
+// programmatic dependent launch.
+//
+// Every such kernel calls chain_begin() before it touches global memory: it
+// lets the next kernel of the stream be set up (its CTAs take their places as
+// these leave) and waits until the kernels before it have finished and their
+// writes are visible.  A run of them saves the 2 us that a launch after a
+// finished kernel costs; after a kernel that does not take part the wait is
+// over at once.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace s2b {
+
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void chain_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void chain_begin() {
+    chain_release();
+    chain_wait();
+}
+
+// True when the launch was accepted.  cluster: CTAs a cluster (0: none).
+template <typename... P, typename... A>
+bool launch_chained(void (*f)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t s, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, f, static_cast<P>(args)...) == cudaSuccess;
+}
+
+}  // namespace s2b

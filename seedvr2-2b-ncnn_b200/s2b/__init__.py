@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -26,7 +27,11 @@ LIB_PATH = os.path.join(_PKG, "lib", "libs2b.so")
 
 _F32P = ctypes.POINTER(ctypes.c_float)
 _I32P = ctypes.POINTER(ctypes.c_int)
-_L3 = ctypes.c_long * 3
+# s2b_op_packed: operator, context, stream, arguments, zeros up to 24 words
+_QUANT = struct.Struct("@12q96x")
+_LINEAR = struct.Struct("@16q64x")
+_ROPE = struct.Struct("@21q24x")
+_NORM = struct.Struct("@12qd6q40x")
 
 
 class S2BError(RuntimeError):
@@ -123,6 +128,7 @@ def lib() -> ctypes.CDLL:
         "s2b_groupnorm_workspace": [ip, ip, ip, ip, ctypes.POINTER(ctypes.c_size_t)],
         "s2b_groupnorm_dev": [vp, vp, ip, ip, ip, ip, ip, ip, vp, vp, ctypes.c_float, ip, vp, ip, ip, vp,
                               ctypes.c_size_t, vp],
+        "s2b_op_packed": [ctypes.c_char_p],
         "s2b_synth_write_m5": [ctypes.c_char_p, u64, ip, ip],
         "s2b_synth_vid_grid": [_F32P, ip, ip, ip, u64],
         "s2b_synth_txt": [_F32P, ip, u64],
@@ -393,11 +399,13 @@ class DitB200:
         rc = lib().s2b_ctx_create(device, precision, ctypes.byref(self._ctx))
         _check(None, rc)
         self.precision = precision
+        self._h, self._op = self._ctx.value, lib().s2b_op_packed     # of the operators' short calls
 
     def close(self):
         if self._ctx:
             lib().s2b_ctx_destroy(self._ctx)
             self._ctx = ctypes.c_void_p()
+            self._h = 0
 
     def __del__(self):
         try:
@@ -460,26 +468,36 @@ class DitB200:
     def fp8_quant_dev(self, d_x: int, x_type: int, rows: int, cols: int, ldx: int, block_rows: int, d_q: int, ldq: int,
                       d_scale: int, stream: int):
         """e4m3 codes and scales of x in blocks of 128 columns x 1 or 128 rows (s2b_fp8_quant_dev)."""
-        self._c(lib().s2b_fp8_quant_dev(self._ctx, d_x, x_type, rows, cols, ldx, block_rows, d_q, ldq, d_scale, stream))
+        rc = self._op(_QUANT.pack(0, self._h, stream, d_x or 0, x_type, rows, cols, ldx, block_rows, d_q or 0, ldq,
+                                  d_scale or 0))
+        if rc:
+            self._c(rc)
 
     def linear_fp8_dev(self, d_xq: int, ldx: int, d_xs: int, M: int, K: int, d_wq: int, ldw: int, d_ws: int, N: int,
                        d_bias, d_y: int, y_type: int, ldy: int, stream: int):
         """y = (xq . xs) (wq . ws)^T (+ bias) on 8-bit codes (s2b_linear_fp8_dev)."""
-        self._c(lib().s2b_linear_fp8_dev(self._ctx, d_xq, ldx, d_xs, M, K, d_wq, ldw, d_ws, N, d_bias, d_y, y_type,
-                                         ldy, stream))
+        rc = self._op(_LINEAR.pack(1, self._h, stream, d_xq or 0, ldx, d_xs or 0, M, K, d_wq or 0, ldw, d_ws or 0, N,
+                                   d_bias or 0, d_y or 0, y_type, ldy))
+        if rc:
+            self._c(rc)
 
     def rope_dev(self, plan: s2b_rope, d_x: int, x_type: int, batch: int, tokens: int, heads: int, head_dim: int,
                  x_strides, d_pos, pos_batch_stride: int, pos0: int, d_y: int, y_strides, inverse: bool, stream: int):
         """Rotary positions (s2b_rope_dev); strides are (batch, token, head) in elements."""
-        self._c(lib().s2b_rope_dev(self._ctx, plan, d_x, x_type, batch, tokens, heads, head_dim, _L3(*x_strides),
-                                   d_pos, pos_batch_stride, pos0, d_y, _L3(*y_strides), bool(inverse), stream))
+        rc = self._op(_ROPE.pack(2, self._h, stream, ctypes.addressof(plan), d_x or 0, x_type, batch, tokens, heads,
+                                 head_dim, *x_strides, d_pos or 0, pos_batch_stride, pos0, d_y or 0, *y_strides,
+                                 1 if inverse else 0))
+        if rc:
+            self._c(rc)
 
     def groupnorm_dev(self, d_x: int, x_type: int, batch: int, rows: int, channels: int, ldx: int, groups: int, d_gamma,
                       d_beta, eps: float, act: int, d_y: int, y_type: int, ldy: int, d_work, work_bytes: int,
                       stream: int):
         """GroupNorm (+ SiLU) over channel-last rows (s2b_groupnorm_dev)."""
-        self._c(lib().s2b_groupnorm_dev(self._ctx, d_x, x_type, batch, rows, channels, ldx, groups, d_gamma, d_beta,
-                                        eps, act, d_y, y_type, ldy, d_work, work_bytes, stream))
+        rc = self._op(_NORM.pack(3, self._h, stream, d_x or 0, x_type, batch, rows, channels, ldx, groups, d_gamma or 0,
+                                 d_beta or 0, eps, act, d_y or 0, y_type, ldy, d_work or 0, work_bytes))
+        if rc:
+            self._c(rc)
 
     def forward_grid(self, vid_grid, txt, TXT, timestep=1000.0):
         T, H, W, _ = vid_grid.shape

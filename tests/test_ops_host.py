@@ -173,3 +173,29 @@ def test_rope_plan_python_refusals():
     for kw in (dict(axis_dims=[]), dict(axis_dims=[2] * 4), dict(axis_dims=[64], layout="x"), dict(axis_dims=[64], scaling="x")):
         with pytest.raises(ValueError):
             s2b.rope_plan(**kw)
+
+
+def packed(op, *words):
+    import struct
+    return s2b.lib().s2b_op_packed(struct.pack("@24q", *([op, 0, 0] + [w or 0 for w in words] + [0] * (21 - len(words)))))
+
+
+def test_packed_calls_are_checked_like_the_others():
+    plan = s2b.rope_plan([64])
+    at = ctypes.addressof(plan)
+    refused(packed(0, X, 3, 4, 256, 256, 1, Q, 256, S), "x_type")
+    refused(packed(0, X, BF16, 4, 256, 256, 1, Q, 256, S), "null context")
+    refused(packed(1, X, 256, S, 4, 0, W, 256, V, 64, 0, Y, BF16, 64), "K must be positive")
+    refused(packed(1, X, 256, S, 4, 256, W, 256, V, 64, 0, Y, BF16, 64), "null context")
+    refused(packed(2, at, X, BF16, 2, 3, 4, 62, 1536, 512, 128, 0, 0, 0, Y, 1536, 512, 128, 0), "more than head_dim")
+    refused(packed(2, at, X, BF16, 2, 3, 4, 128, 1536, 512, 128, 0, 0, 0, Y, 1536, 512, 128, 0), "null context")
+    eps = np.array([1e-6]).view(np.int64)[0]
+    refused(packed(3, X, BF16, 2, 10, 64, 64, 7, S, V, eps, 1, Y, BF16, 64, B, 1 << 19), "multiple of groups")
+    refused(packed(3, X, BF16, 2, 10, 64, 64, 8, S, V, eps, 1, Y, BF16, 64, B, 1 << 19), "null context")
+    refused(packed(4), "unknown operator")
+    refused(s2b.lib().s2b_op_packed(None), "null argument")
+    for bad in (1 << 31, -(1 << 31) - 1, 1 << 40):
+        refused(packed(0, X, BF16, bad, 256, 256, 1, Q, 256, S), "out of range")
+        refused(packed(1, X, 256, S, 4, 256, W, 256, V, bad, 0, Y, BF16, 64), "out of range")
+        refused(packed(2, at, X, BF16, 2, bad, 4, 128, 1536, 512, 128, 0, 0, 0, Y, 1536, 512, 128, 0), "out of range")
+        refused(packed(3, X, BF16, 2, bad, 64, 64, 8, S, V, eps, 1, Y, BF16, 64, B, 1 << 19), "out of range")
