@@ -364,7 +364,7 @@ struct alignas(16) PairCtl {
 
 struct PairTiles {
     int num_m, num_n, total;
-    int tma_y;                           // y through TMA boxes (16-byte rows)
+    int tma_y, tma_edge;                 // y through TMA boxes (16-byte rows); the last columns too
 };
 
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; }
@@ -411,12 +411,14 @@ __device__ __forceinline__ void stage_chunk(uint8_t* box, const uint32_t v[32], 
 }
 
 // The warp's staged box of 32 columns from column c to y: one TMA store, or
-// element by element where y's rows start on no 16 bytes.
+// element by element where y's rows start on no 16 bytes, and in the last
+// columns where y's width is no multiple of 16 bytes (the store writes whole
+// 16-byte pieces, past the tensor map's width).
 __device__ __forceinline__ void flush_chunk(const LinParams& P, const PairTiles& T, const CUtensorMap* my, const uint8_t* box, int row0,
                                             int c) {
     const int lane = threadIdx.x & 31;
     if (row0 >= P.M || c >= P.N) return;
-    if (T.tma_y) {
+    if (T.tma_y && (T.tma_edge || c + 32 <= P.N)) {
         if (lane == 0) sm100::tma_store_2d(my, box, c, row0);
         return;
     }
@@ -799,6 +801,7 @@ int launch_pair(const Fp8LinearArgs& a, const LinParams& P, cudaStream_t s) {
     T.total = (int)tiles;
     const size_t e = a.y_type == S2B_PREC_FP32 ? 4 : 2;
     T.tma_y = ((uintptr_t)a.y & 15) == 0 && (size_t)a.ldy * e % 16 == 0;
+    T.tma_edge = (size_t)a.N * e % 16 == 0;
     if (T.tma_y) {
         if (!make_tmap_out(&my, a.y, a.y_type, a.M, a.N, a.ldy)) return -1;
     } else {

@@ -226,14 +226,16 @@ int launch(const RopeArgs& a, cudaStream_t s) {
 template <typename T>
 int launch_t(const RopeArgs& a, cudaStream_t s) {
     // 16-byte pieces where every head starts on one and neither layout cuts
-    // a piece in two; single elements otherwise
+    // a piece in two, pieces of two elements likewise, single elements otherwise
+    auto fits = [&](int v) {
+        bool ok = (uintptr_t)a.x % (v * sizeof(T)) == 0 && (uintptr_t)a.y % (v * sizeof(T)) == 0 && a.head_dim % v == 0 &&
+                  (!a.plan->half || a.plan->pairs % v == 0);
+        const long n[3] = {a.batch, a.tokens, a.heads};
+        for (int i = 0; i < 3; i++) ok = ok && (n[i] <= 1 || (a.xs[i] % v == 0 && a.ys[i] % v == 0));
+        return ok;
+    };
     constexpr int V = 16 / (int)sizeof(T);
-    bool ok = ((uintptr_t)a.x & 15) == 0 && ((uintptr_t)a.y & 15) == 0 && a.head_dim % V == 0 &&
-              (!a.plan->half || a.plan->pairs % V == 0);
-    const long n[3] = {a.batch, a.tokens, a.heads};
-    for (int i = 0; i < 3; i++)
-        if (n[i] > 1 && (a.xs[i] % V || a.ys[i] % V)) ok = false;
-    return ok ? launch<T, V>(a, s) : launch<T, 1>(a, s);
+    return fits(V) ? launch<T, V>(a, s) : fits(2) ? launch<T, 2>(a, s) : launch<T, 1>(a, s);
 }
 
 }  // namespace

@@ -200,7 +200,8 @@ def test_linear_vs_64bit(ctx, M, K, N, t):
     check_linear(run_linear(ctx, xq, xs, wq, ws, K, bias, t), M, N, ref, mag, K, t)
 
 
-@pytest.mark.parametrize("M,K,N,ldy", [(3, 300, 200, 208), (70, 256, 130, 133), (700, 512, 640, 648), (700, 512, 600, 603)])
+@pytest.mark.parametrize("M,K,N,ldy", [(3, 300, 200, 208), (70, 256, 130, 133), (700, 512, 640, 648), (700, 512, 600, 603), (1400, 300, 1300, 1304),
+                                       (1400, 1100, 1303, 1304)])
 def test_linear_any_scales_and_pitches(ctx, M, K, N, ldy):
     """Scales that are no powers of two, among them 0, negative and far apart ones; codes inside wider rows whose rest is
     NaN; y inside wider rows."""
@@ -219,7 +220,43 @@ def test_linear_any_scales_and_pitches(ctx, M, K, N, ldy):
         check_linear(run_linear(ctx, xq, xs, wq, ws, K, bias, t, ldy), M, N, ref, mag, K, t)
 
 
-@pytest.mark.parametrize("M,N", [(1, 256), (40, 300), (600, 512)])
+# sizes that the CTA-pair kernel takes: odd numbers of blocks, one block, rows of y off 16 bytes, both tile widths
+PAIR_SHAPES = [(1500, 128, 1000), (700, 300, 2000), (2049, 640, 1281), (300, 1664, 4000), (1400, 16, 1300), (4200, 900, 776), (900, 2200, 2563)]
+
+
+@pytest.mark.parametrize("M,K,N", PAIR_SHAPES)
+@pytest.mark.parametrize("t", [FP32, BF16], ids=IDS)
+def test_linear_many_rows_scaled_general_and_mixed(ctx, M, K, N, t):
+    """Scales that are powers of two, scales that are none, and a few of these among those (so that some tiles of a call
+    run one way and some the other), each with bias and with the rows of y inside wider ones."""
+    g = gen(M + N)
+    kb = -(-K // 128)
+    xq, xs = codes(normal(g, M, K) * torch.exp(normal(g, M, 1)), 1)
+    wq, ws = codes(0.02 * normal(g, N, K), 128)
+    bias = normal(g, N)
+    some = xs.clone()
+    some[0, M // 2], some[kb - 1, 3] = 0.3, 0.0
+    wsome = ws.clone()
+    wsome[ws.shape[0] - 1, 0] = 3.0e-3
+    for a, b in ((xs, ws), (some, ws), (xs, wsome), (xs * 1.1, ws * 0.7)):
+        ref, mag = linear64(xq, a, wq, b, K, bias)
+        for ldy in (N, N + 5):
+            check_linear(run_linear(ctx, xq, a, wq, b, K, bias, t, ldy), M, N, ref, mag, K, t)
+
+
+def test_linear_extreme_scales(ctx):
+    """Scales at both ends of what one byte of exponent holds, and past it (subnormal, zero): products stay fp32's."""
+    M, K, N = 1500, 256, 1024
+    g = gen(77)
+    xq, xs = codes(normal(g, M, K), 1)
+    wq, ws = codes(normal(g, N, K), 128)
+    for ex, ew in ((2.0 ** -126, 2.0 ** 100), (2.0 ** 120, 2.0 ** -126), (2.0 ** -130, 2.0 ** 120), (0.0, 1.0), (2.0 ** 60, 2.0 ** -60)):
+        a, b = torch.full_like(xs, ex), torch.full_like(ws, ew)
+        ref, mag = linear64(xq, a, wq, b, K, None)
+        check_linear(run_linear(ctx, xq, a, wq, b, K, None, FP32), M, N, ref, mag, K, FP32)
+
+
+@pytest.mark.parametrize("M,N", [(1, 256), (40, 300), (600, 512), (1700, 1280)])
 def test_linear_nan_stays_in_its_row_and_column(ctx, M, N):
     g, K = gen(9), 700
     xq, xs = codes(normal(g, M, K), 1)
