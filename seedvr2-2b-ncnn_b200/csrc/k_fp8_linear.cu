@@ -347,7 +347,7 @@ static_assert(P_REGS_0 + P_REGS_1 + 2 * P_REGS_EPI <= 4 * P_REGS, "register shar
 template <int BN> struct PairCfg8 {
     static constexpr int CH = BN / 32, CH0 = (CH + 1) / 2;       // chunks of a tile, of warpgroup 2
     static constexpr int A_TILE = 128 * KB, B_TILE = BN / 2 * KB, STAGE = A_TILE + B_TILE;
-    static constexpr int BOX = 4096;                             // a warp's staging: 2 chunks of 16-bit y, 1 of fp32
+    static constexpr int BOX = 4096;                             // a warp's staging: two boxes of 16-bit y, one of fp32
     static constexpr int SMEM = PSTAGES * STAGE + 8 * BOX + 1024 + 1024;
     static constexpr int SF = 2 * BN;                            // TMEM column of the scale bytes: RING x 16
     static_assert(SF + RING * 16 <= 512 && BN % 32 == 0 && CH <= 8 && STAGE % 1024 == 0, "TMEM and tile layout");
@@ -690,12 +690,13 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
         sm100::regs_grow<P_REGS_EPI>();
         const int side = wg - 2, c0 = side * C::CH0, nc = side ? C::CH - C::CH0 : C::CH0;      // this warp's chunks
         uint8_t* box = boxes + (warp - 8) * C::BOX;
-        const int per_box = P.y_type == S2B_PREC_FP32 ? 4096 : 2048, group = P.y_type == S2B_PREC_FP32 ? 1 : 2;
+        const int per_box = P.y_type == S2B_PREC_FP32 ? 4096 : 2048, boxes_n = C::BOX / per_box;
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + c0 * 32;
         uint32_t tempty[2];
         tempty[0] = sm100::map_to_rank(&ctl->tempty[0], 0);
         tempty[1] = sm100::map_to_rank(&ctl->tempty[1], 0);
         uint32_t use = 0, ti = 0;
+        int put = 0;                     // the staging box that comes next
         bool ok = true;
         for (int tile = pair; tile < T.total && ok; tile += npairs, ti++) {
             const int row0 = tile % T.num_m * PBM + (int)rank * 128 + q * 32, n0 = tile / T.num_m * BN + c0 * 32;
@@ -712,31 +713,43 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
                 const int nwb = (P.N + KB - 1) / KB;
                 // chunk c is in weight block n0 / KB + step(c)
                 auto step = [&](int c) { return (n0 % KB + 32 * c) / KB; };
-                float x1 = px ? __ldg(px) : 0.f;
+                // scales two blocks ahead of their use
+                struct Scale { float x, w[2]; };
+                auto scale = [&](int kb) {
+                    Scale v = {0.f, {0.f, 0.f}};
+                    if (kb >= P.nkb) return v;
+                    if (px) v.x = __ldg(px + (size_t)kb * P.M);
+                    v.w[0] = n0 / KB < nwb ? __ldg(pw + kb) : 0.f;
+                    v.w[1] = n0 / KB + 1 < nwb ? __ldg(pw + P.nkb + kb) : 0.f;
+                    return v;
+                };
+                Scale v0 = scale(0), v1 = scale(1);
                 for (int kb = 0; kb < P.nkb; kb++, use++) {
-                    const float x = x1;
-                    if (px && kb + 1 < P.nkb) x1 = __ldg(px + (size_t)(kb + 1) * P.M);
-                    float w[2];
-                    #pragma unroll
-                    for (int j = 0; j < 2; j++) w[j] = n0 / KB + j < nwb ? __ldg(pw + (size_t)j * P.nkb + kb) : 0.f;
-                    const uint32_t slot = use & 1;
+                    const float s0 = v0.x * v0.w[0], s1 = v0.x * v0.w[1];
+                    v0 = v1;
+                    v1 = scale(kb + 2);
+                    const uint32_t slot = use & 1, ta = taddr + slot * BN;
                     if (!__all_sync(0xffffffffu, wait_flag(&ctl->tfull[slot], (use >> 1) & 1, abort_flag, P.flag))) { ok = false; break; }
                     sm100::tc_fence_after();
+                    // 16 columns on their way while 16 are added
+                    uint32_t d[2][16];
+                    sm100::tmem_ld16_async(ta, d[0]);
                     #pragma unroll
-                    for (int c = 0; c < C::CH0; c++) {
-                        if (c >= nc) break;
-                        uint32_t d[32];
-                        sm100::tmem_ld32_async(taddr + slot * BN + 32 * c, d);
-                        sm100::tmem_wait32(d);
-                        if (c == nc - 1) {       // the slot is read: back to the MMA warp
+                    for (int c = 0; c < 2 * C::CH0; c++) {
+                        if (c >= 2 * nc) break;
+                        sm100::tmem_wait16(d[c & 1]);
+                        if (c + 1 < 2 * nc) {
+                            sm100::tmem_ld16_async(ta + 16 * (c + 1), d[(c + 1) & 1]);
+                        } else {                 // the slot is read: back to the MMA warp
                             sm100::tc_fence_before();
                             __syncwarp();
                             if (lane == 0) sm100::mbar_arrive_cluster_cta(slot ? tempty[1] : tempty[0]);
                         }
-                        const uint32_t sb = __float_as_uint(x * (step(c) ? w[1] : w[0]));
+                        const uint32_t sb = __float_as_uint(step(c / 2) ? s1 : s0);
                         const uint64_t ss = pack2(sb, sb);
                         #pragma unroll
-                        for (int i = 0; i < 16; i++) acc[c][i] = fma2(pack2(d[2 * i], d[2 * i + 1]), ss, acc[c][i]);
+                        for (int i = 0; i < 8; i++)
+                            acc[c / 2][c % 2 * 8 + i] = fma2(pack2(d[c & 1][2 * i], d[c & 1][2 * i + 1]), ss, acc[c / 2][c % 2 * 8 + i]);
                     }
                 }
                 if (!ok) break;
@@ -763,19 +776,20 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
                 }
                 const int col = n0 + 32 * c;
                 const float bias = P.bias && col + lane < P.N ? __ldg(P.bias + col + lane) : 0.f;
-                if (c % group == 0) {            // the staging's previous stores have been read
-                    if (lane == 0) sm100::bulk_wait_read_all();
-                    __syncwarp();
+                // the box's previous store has been read
+                uint8_t* st = box + put * per_box;
+                put = (put + 1) % boxes_n;
+                if (lane == 0) {
+                    if (boxes_n == 2) sm100::bulk_wait_read<1>();
+                    else sm100::bulk_wait_read<0>();
                 }
-                if (P.bias) stage_chunk<true>(box + c % group * per_box, d, bias, P.y_type);
-                else stage_chunk<false>(box + c % group * per_box, d, 0.f, P.y_type);
-                if (c % group == group - 1 || c == nc - 1) {
-                    if (T.tma_y) sm100::fence_proxy_async_smem();
-                    __syncwarp();
-                    for (int k = c - c % group; k <= c; k++) flush_chunk(P, T, &my, box + k % group * per_box, row0, n0 + 32 * k);
-                    if (T.tma_y && lane == 0) sm100::bulk_commit_group();
-                    __syncwarp();
-                }
+                __syncwarp();
+                if (P.bias) stage_chunk<true>(st, d, bias, P.y_type);
+                else stage_chunk<false>(st, d, 0.f, P.y_type);
+                if (T.tma_y) sm100::fence_proxy_async_smem();
+                __syncwarp();
+                flush_chunk(P, T, &my, st, row0, col);
+                if (lane == 0) sm100::bulk_commit_group();
             }
             if (way) use++;
         }
