@@ -637,6 +637,59 @@ def test_front_captured_and_replayed_on_new_inputs(ctx):
             assert torch.equal(f.y, y)
 
 
+# ---------------------------------------------------------------- far offsets, broadcasts
+def test_offsets_past_32_bits(ctx):
+    """Rows, samples and heads that start more than 2^32 elements (or bytes) into their buffers."""
+    g = gen(31)
+    far = (1 << 32) + 1024
+    # rotary: the second sample far away, in and out
+    plan = s2b.rope_plan([128], layout="half")
+    big, out = (torch.empty(far + 4096, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    x, y = (torch.as_strided(b, (2, 3, 2, 128), (far, 256, 128, 1)) for b in (big, out))
+    x.copy_(normal(g, 2, 3, 2, 128))
+    run_rope(ctx, plan, x, BF16, None, 0, 5, y)
+    pos = (torch.arange(3, device=DEV) + 5)[None, :, None].expand(2, 3, 1)
+    ref, mag = rope64(plan, x.contiguous(), pos, False)
+    check_rope(y, ref, mag, BF16, 10, plan)
+    # GroupNorm: rows 2^17 apart, streamed and in place
+    S, C, ld = 40000, 64, 1 << 17
+    assert S * ld > 1 << 32
+    del big, out, x, y
+    buf = torch.empty(S * ld // 2 + C, dtype=torch.bfloat16, device=DEV)
+    x = torch.as_strided(buf, (1, S, C), (S * ld // 2, ld // 2, 1))
+    x.copy_(normal(g, 1, S, C))
+    keep = x.contiguous()
+    run_norm(ctx, x, 8, None, None, 1e-6, False, BF16, y=x)
+    check_norm(x.contiguous(), keep, 8, None, None, 1e-6, False, BF16)
+    # quantisation: codes and rows far apart
+    x = torch.as_strided(buf, (S, 32), (ld // 2, 1))
+    x.copy_(normal(g, S, 32))
+    q = torch.empty(S * ld, dtype=torch.uint8, device=DEV)
+    s = torch.empty(1, S, device=DEV)
+    ctx.fp8_quant_dev(x.data_ptr(), BF16, S, 32, ld // 2, 1, q.data_ptr(), ld, s.data_ptr(), stream())
+    qr, sr = quantise64(x.contiguous(), 1)
+    codes_ = torch.as_strided(q, (S, 32), (ld, 1)).contiguous()
+    assert torch.equal(decode(codes_), qr) and torch.equal(s.double(), sr)
+    # Linear: those codes as x, y's rows far apart, by both kernels
+    wq, ws = codes(normal(g, 1000, 32), 128)
+    for M in (40, 36000):
+        ref, mag = linear64(codes_[:M], s[:, :M].contiguous(), wq, ws, 32, None)
+        xs = s[:, :M].contiguous()
+        ctx.linear_fp8_dev(q.data_ptr(), ld, xs.data_ptr(), M, 32, wq.data_ptr(), wq.stride(0), ws.data_ptr(), 1000, None,
+                           buf.data_ptr(), BF16, ld // 2, stream())
+        y = torch.as_strided(buf, (M, 1000), (ld // 2, 1)).double()
+        assert ((y - ref).abs() <= 40 * 2.0 ** -23 * mag + HALF[BF16] * ref.abs() + TINY[BF16]).all()
+
+
+def test_rope_broadcast_heads(ctx):
+    """One head read for many (stride 0), as shared keys are: the gradient's inverse takes the heads apart again."""
+    plan = s2b.rope_plan([64], layout="half")
+    x = normal(gen(3), 1, 40, 1, 64)
+    y = run_rope(ctx, plan, x.expand(1, 40, 6, 64), FP32, None, 0, 0, torch.empty(1, 40, 6, 64, device=DEV))
+    one = run_rope(ctx, plan, x, FP32, None, 0, 0, torch.empty_like(x))
+    assert torch.equal(y, one.expand(1, 40, 6, 64))
+
+
 # ---------------------------------------------------------------- refusals that need the context
 def test_host_memory_is_refused_and_writes_nothing(ctx):
     h = torch.zeros(16, 128)
