@@ -221,7 +221,8 @@ def test_linear_any_scales_and_pitches(ctx, M, K, N, ldy):
 
 
 # sizes that the CTA-pair kernel takes: odd numbers of blocks, one block, rows of y off 16 bytes, both tile widths
-PAIR_SHAPES = [(1500, 128, 1000), (700, 300, 2000), (2049, 640, 1281), (300, 1664, 4000), (1400, 16, 1300), (4200, 900, 776), (900, 2200, 2563)]
+PAIR_SHAPES = [(1500, 128, 1000), (700, 300, 2000), (2049, 640, 1281), (300, 1664, 4000), (1400, 16, 1300), (4200, 900, 776), (900, 2200, 2563),
+               (2600, 640, 13824), (5000, 384, 9000)]            # nine and eleven tiles a pair of CTAs
 
 
 @pytest.mark.parametrize("M,K,N", PAIR_SHAPES)
@@ -238,6 +239,7 @@ def test_linear_many_rows_scaled_general_and_mixed(ctx, M, K, N, t):
     some[0, M // 2], some[kb - 1, 3] = 0.3, 0.0
     wsome = ws.clone()
     wsome[ws.shape[0] - 1, 0] = 3.0e-3
+    wsome[:: 7, kb // 2] *= 1.3
     for a, b in ((xs, ws), (some, ws), (xs, wsome), (xs * 1.1, ws * 0.7)):
         ref, mag = linear64(xq, a, wq, b, K, bias)
         for ldy in (N, N + 5):
