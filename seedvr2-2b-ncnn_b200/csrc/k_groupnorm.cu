@@ -22,8 +22,8 @@
 //             normalisation, which reads x again, last chunk first: what the
 //             statistics read last is still in L2.
 //
-// B200: on chip 1360 x 512 bf16 6.7 us; streamed 3 x 21760 x 512 (134 MB read and
-// written once) 40 us, 1392640 x 128 with SiLU (713 MB, of which x twice) 200 us,
+// B200: on chip 1360 x 512 bf16 6.6 us; streamed 3 x 21760 x 512 (134 MB read and
+// written once) 41 us, 1392640 x 128 with SiLU (713 MB, x read twice) 200 us,
 // 184 without: 5.4 TB/s of what DRAM has to move.
 #include "kcommon.cuh"
 #include "launch.cuh"
