@@ -285,8 +285,8 @@ int s2b_fp8_quant_dev(s2b_ctx* ctx, const void* d_x, int x_type, int rows, int c
  * (multiples of 16, bases 16-byte aligned), scales laid out as
  * s2b_fp8_quant_dev writes them for block_rows 1 and 128; they may be any fp32
  * values whose product is one (0 and powers of two included), from any
- * quantiser.  bias (N) or NULL.  y (M, N) of y_type, row pitch ldy.  Any M, N,
- * K > 0; one row to thousands.  Sums are fp32, rounded once to y_type; a NaN
+ * quantiser.  bias (N) or NULL.  y (M, N) of y_type, row pitch ldy.  M, N and
+ * K > 0 up to 2^30; one row to thousands.  Sums are fp32, rounded once to y_type; a NaN
  * code makes the outputs that it enters NaN.  y must not overlap an operand.
  * A bounded wait that expires is reported by s2b_check_errors. */
 int s2b_linear_fp8_dev(s2b_ctx* ctx, const void* d_xq, int ldx, const float* d_xs, int M, int K, const void* d_wq,
@@ -337,7 +337,8 @@ int s2b_rope_plan(const s2b_rope_config* config, s2b_rope* plan);
  * y likewise.  Position of a token on axis a: d_pos[b * pos_batch_stride +
  * t * axes + a] (int32, any value; stride 0 shares them between samples), or
  * pos0 + t on every axis when d_pos is NULL.  y may be x with the same strides;
- * otherwise the two must not overlap.  Angles are exact to 2^-32 of a turn at
+ * otherwise the two, from first to last value, must not overlap.  No buffer
+ * may reach over more than 2^40 values.  Angles are exact to 2^-32 of a turn at
  * every position. */
 int s2b_rope_dev(s2b_ctx* ctx, const s2b_rope* plan, const void* d_x, int type, int batch, int tokens, int heads,
                  int head_dim, const long x_strides[3], const int* d_pos, long pos_batch_stride, int pos0, void* d_y,
@@ -352,7 +353,7 @@ int s2b_rope_dev(s2b_ctx* ctx, const s2b_rope* plan, const void* d_x, int type, 
  * same type and pitch; otherwise they must not overlap.  d_work: device
  * workspace of s2b_groupnorm_workspace bytes (16-byte aligned), contents
  * arbitrary before and after; two calls that may run at the same time need one
- * each. */
+ * each.  Up to 65535 samples, 2^30 rows and 2^23 channels. */
 #define S2B_ACT_NONE 0
 #define S2B_ACT_SILU 1
 int s2b_groupnorm_workspace(int batch, int rows, int channels, int groups, size_t* bytes);

@@ -361,6 +361,7 @@ int s2b_groupnorm_workspace(int batch, int rows, int channels, int groups, size_
     if (!bytes) return refuse(nullptr, S2B_ERR_ARG, "groupnorm: null argument");
     if (batch < 0 || rows < 0 || channels <= 0 || groups <= 0)
         return refuse(nullptr, S2B_ERR_ARG, "groupnorm: batch and rows must not be negative, channels and groups must be positive");
+    if (const char* why = s2b::groupnorm_limits(batch, rows, channels)) return refuse(nullptr, S2B_ERR_ARG, why);
     *bytes = s2b::groupnorm_workspace(batch, rows, channels, groups);
     return S2B_OK;
 }

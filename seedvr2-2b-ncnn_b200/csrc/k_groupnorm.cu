@@ -368,10 +368,10 @@ int chunk_rows(long batch, int rows, int per_sm, int round) {
 // then larger while the GPU has idle SMs and a CTA more than 32 rows.
 bool plan_chip(const GroupNormArgs& a, int vec, int xe, GnParams& P, int& rv) {
     P.slab = 0;
-    for (int k = 1; k <= P.G; k++) {
+    for (int k = 1; k <= P.G && k <= CHIP_GROUPS; k++) {
         const long w = (long)k * P.cpg;
         if (P.G % k || w % vec || (w * xe < 64 && w < P.C)) continue;
-        if (k > CHIP_GROUPS || w / vec > THREADS) break;
+        if (w / vec > THREADS) break;
         P.slab = (int)w;
         break;
     }

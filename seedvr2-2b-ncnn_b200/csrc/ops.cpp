@@ -9,7 +9,8 @@ namespace {
 
 inline bool type_ok(int t) { return t == S2B_PREC_FP32 || t == S2B_PREC_FP16 || t == S2B_PREC_BF16; }
 inline int type_bytes(int t) { return t == S2B_PREC_FP32 ? 4 : 2; }
-constexpr long MAX_STRIDE = 1L << 40;   // elements; keeps every span below 2^63 bytes
+constexpr long MAX_STRIDE = 1L << 40;   // elements
+constexpr int MAX_SIZE = 1 << 30;       // tile arithmetic stays in 32 bits
 
 inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
@@ -20,6 +21,9 @@ inline bool overlap(const void* p, size_t bytes, const void* q, size_t more) {
 }
 // bytes from the first to the last element of rows x cols with a row pitch
 inline size_t span(size_t rows, size_t cols, size_t ld, size_t e) { return rows ? ((rows - 1) * ld + cols) * e : 0; }
+// n steps of a stride reach further than any memory, and than 64-bit offsets
+// can be trusted with (both not negative).
+inline bool too_far(long n, long stride) { return n > 1 && stride > MAX_STRIDE / (n - 1); }
 
 }  // namespace
 
@@ -43,6 +47,7 @@ const char* op_check(const Fp8QuantArgs& a) {
 const char* op_check(const Fp8LinearArgs& a) {
     if (!type_ok(a.y_type)) return "fp8 linear: y_type must be S2B_PREC_FP32, _FP16 or _BF16";
     if (a.M < 0 || a.N < 0 || a.K <= 0) return "fp8 linear: M and N must not be negative, K must be positive";
+    if (a.M > MAX_SIZE || a.N > MAX_SIZE || a.K > MAX_SIZE) return "fp8 linear: M, N or K above 2^30";
     if (op_empty(a)) return nullptr;
     if (!a.xq || !a.xs || !a.wq || !a.ws || !a.y) return "fp8 linear: null buffer";
     if (a.ldx < a.K || a.ldw < a.K || a.ldy < a.N) return "fp8 linear: row pitch below the row's length";
@@ -62,6 +67,7 @@ const char* op_check(const RopeArgs& a) {
     if (!type_ok(a.type)) return "rope: type must be S2B_PREC_FP32, _FP16 or _BF16";
     if (a.batch < 0 || a.tokens < 0 || a.heads < 0 || a.head_dim <= 0)
         return "rope: batch, tokens and heads must not be negative, head_dim must be positive";
+    if (a.head_dim > MAX_SIZE) return "rope: head_dim above 2^30";
     if (!a.plan) return "rope: null plan";
     const s2b_rope& p = *a.plan;
     if (p.pairs < 0 || p.pairs > S2B_ROPE_MAX_PAIRS || p.axes < 1 || p.axes > 3 || (p.half != 0 && p.half != 1) ||
@@ -78,9 +84,12 @@ const char* op_check(const RopeArgs& a) {
         if (a.xs[i] < 0 || a.ys[i] < 0 || a.xs[i] > MAX_STRIDE || a.ys[i] > MAX_STRIDE)
             return "rope: stride negative or above 2^40";
     if (a.pos && (a.pos_bs < 0 || a.pos_bs > MAX_STRIDE)) return "rope: stride negative or above 2^40";
+    const long D = a.head_dim, n[3] = {a.batch, a.tokens, a.heads};
+    for (int i = 0; i < 3; i++)
+        if (too_far(n[i], a.xs[i]) || too_far(n[i], a.ys[i])) return "rope: x or y reaches over more than 2^40 values";
+    if (a.pos && too_far(a.batch, a.pos_bs)) return "rope: the positions reach over more than 2^40 values";
     // y is written by many threads at once: no two of its heads may share an
     // element, whichever order the three strides nest in
-    const long D = a.head_dim, n[3] = {a.batch, a.tokens, a.heads};
     int ord[3] = {0, 1, 2};
     for (int i = 0; i < 3; i++)
         for (int j = i + 1; j < 3; j++)
@@ -106,6 +115,11 @@ const char* op_check(const RopeArgs& a) {
     return nullptr;
 }
 
+const char* groupnorm_limits(int batch, int rows, int channels) {
+    return batch > 65535 || rows > MAX_SIZE || channels > 1 << 23
+               ? "groupnorm: more than 65535 samples, 2^30 rows or 2^23 channels" : nullptr;
+}
+
 const char* op_check(const GroupNormArgs& a) {
     if (!type_ok(a.x_type) || !type_ok(a.y_type)) return "groupnorm: types must be S2B_PREC_FP32, _FP16 or _BF16";
     if (a.batch < 0 || a.rows < 0 || a.channels <= 0 || a.groups <= 0)
@@ -113,7 +127,7 @@ const char* op_check(const GroupNormArgs& a) {
     if (a.channels % a.groups) return "groupnorm: channels must be a multiple of groups";
     if (a.act != 0 && a.act != 1) return "groupnorm: act must be S2B_ACT_NONE or S2B_ACT_SILU";
     if (!(a.eps >= 0.f) || !std::isfinite(a.eps)) return "groupnorm: eps must be finite and not negative";
-    if (a.batch > 65535 || a.rows > (1 << 30)) return "groupnorm: more than 65535 samples or 2^30 rows";
+    if (const char* why = groupnorm_limits(a.batch, a.rows, a.channels)) return why;
     if (op_empty(a)) return nullptr;
     if (!a.x || !a.y) return "groupnorm: null buffer";
     if (a.ldx < a.channels || a.ldy < a.channels) return "groupnorm: row pitch below channels";

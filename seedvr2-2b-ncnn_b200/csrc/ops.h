@@ -67,6 +67,7 @@ int op_launch(const GroupNormArgs& a, cudaStream_t s);
 // Rotary frequencies of a configuration; null, or why it is refused.
 const char* rope_plan(const s2b_rope_config& c, s2b_rope* out);
 // Bytes of device workspace of a GroupNorm call; 0 when it needs none.
+const char* groupnorm_limits(int batch, int rows, int channels);
 size_t groupnorm_workspace(int batch, int rows, int channels, int groups);
 
 // SMs of the current device (148 when it was not initialised).

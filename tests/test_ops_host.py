@@ -199,3 +199,25 @@ def test_packed_calls_are_checked_like_the_others():
         refused(packed(1, X, 256, S, 4, 256, W, 256, V, bad, 0, Y, BF16, 64), "out of range")
         refused(packed(2, at, X, BF16, 2, bad, 4, 128, 1536, 512, 128, 0, 0, 0, Y, 1536, 512, 128, 0), "out of range")
         refused(packed(3, X, BF16, 2, bad, 64, 64, 8, S, V, eps, 1, Y, BF16, 64, B, 1 << 19), "out of range")
+
+
+def test_sizes_past_the_limits_are_refused():
+    """Sizes whose tile counts or offsets would leave their integers."""
+    big, far = 2 ** 31 - 1, 1 << 40
+    refused(linear(M=big), "2^30")
+    refused(linear(N=big, ldy=big), "2^30")
+    refused(linear(K=big, ldx=big - 15, ldw=big - 15), "2^30")
+    refused(linear(M=big, N=0), "2^30")
+    refused(rope(dim=big), "2^30")
+    # 2^40 values a step is a stride, 2^30 such steps wrap a 64-bit offset
+    refused(rope(tokens=2 ** 30, ys=(1536, far, 128)), "reaches over")
+    refused(rope(tokens=2 ** 30, xs=(1536, far, 128)), "reaches over")
+    refused(rope(batch=big, xs=(1 << 33, 512, 128), ys=(1 << 33, 512, 128)), "reaches over")
+    refused(rope(batch=3, pos=Q, pbs=far), "positions reach")
+    refused(rope(batch=1, pos=Q, pbs=far, xs=(far, 512, 128), ys=(far, 512, 128)), "null context")    # no step is taken
+    refused(norm(C=1 << 24, ldx=1 << 24, ldy=1 << 24), "2^23 channels")
+    refused(norm(rows=big), "2^30 rows")
+    for sizes in ((1, big, 64, 8), (65536, 1, 64, 8), (1, 1, big, 1)):
+        with pytest.raises(s2b.S2BError) as e:
+            s2b.groupnorm_workspace(*sizes)
+        assert "more than" in str(e.value)
