@@ -730,3 +730,59 @@ def test_calls_leave_the_current_device(ctx):
     before = torch.cuda.current_device()
     q, s = quantise(ctx, normal(gen(1), 4, 128), 1)
     assert torch.cuda.current_device() == before and ctypes.CDLL(None) is not None
+
+
+# ---------------------------------------------------------------- back to back
+@pytest.mark.parametrize("T,C,N", [(1, 256, 256), (40, 512, 384), (150, 1280, 640), (700, 640, 1280)])
+def test_back_to_back_calls_see_what_the_calls_before_wrote(ctx, T, C, N):
+    """Calls of one stream overlap at their ends.  A run of them over buffers that every step writes anew -- codes and
+    scales, and the weights' scales, bias, gamma and positions, copied by a rotary call without pairs -- gives what the
+    same calls give with the device idle before each; eager and from a graph."""
+    g = gen(T + C)
+    n = 24
+    copy, turned = s2b.rope_plan([0]), s2b.rope_plan([64])
+    nwb, kb = -(-N // 128), -(-C // 128)
+    src = [dict(x=normal(g, T, C).bfloat16(), gamma=normal(g, C), bias=normal(g, N), ws=torch.exp2(torch.randint(-3, 3, (nwb * kb,), generator=g, device=DEV).float()),
+                pos=torch.randint(0, 5000, (T,), generator=g, device=DEV, dtype=torch.int32)) for _ in range(n)]
+    for i in range(0, n, 3):
+        src[i]["ws"] *= 1.25                                   # not powers of two
+    wq, _ = quantise(ctx, normal(g, N, C), 128, ldq=C)
+    now = {k: torch.empty_like(v) for k, v in src[0].items() if k != "x"}
+    work = torch.empty(max(1, s2b.groupnorm_workspace(1, T, C, 32)), dtype=torch.uint8, device=DEV)
+    h = torch.empty(T, C, dtype=torch.bfloat16, device=DEV)
+    xq = torch.empty(T, C, dtype=torch.uint8, device=DEV)
+    xs = torch.empty(kb, T, device=DEV)
+
+    def run(out, idle):
+        st = stream()
+        for i, s in enumerate(src):
+            y = out[i].data_ptr()
+            calls = [lambda k=k: ctx.rope_dev(copy, s[k].data_ptr(), FP32, 1, 1, 1, s[k].numel(), (0, 0, 0), None, 0, 0, now[k].data_ptr(),
+                                              (0, 0, 0), False, st) for k in now]
+            calls += [
+                lambda: ctx.groupnorm_dev(s["x"].data_ptr(), BF16, 1, T, C, C, 32, now["gamma"].data_ptr(), None, 1e-6, s2b.ACT_SILU,
+                                          h.data_ptr(), BF16, C, work.data_ptr(), work.numel(), st),
+                lambda: ctx.fp8_quant_dev(h.data_ptr(), BF16, T, C, C, 1, xq.data_ptr(), C, xs.data_ptr(), st),
+                lambda: ctx.linear_fp8_dev(xq.data_ptr(), C, xs.data_ptr(), T, C, wq.data_ptr(), C, now["ws"].data_ptr(), N,
+                                           now["bias"].data_ptr(), y, BF16, N, st),
+                lambda: ctx.rope_dev(turned, y, BF16, 1, T, N // 64, 64, (0, N, 64), now["pos"].data_ptr(), 0, 0, y, (0, N, 64), False, st)]
+            for c in calls:
+                c()
+                if idle:
+                    torch.cuda.synchronize()
+
+    ref = torch.zeros(n, T, N, dtype=torch.bfloat16, device=DEV)
+    run(ref, True)
+    assert ref.isfinite().all() and not torch.equal(ref[0], ref[1])
+    got = torch.zeros_like(ref)
+    for _ in range(8):
+        got.zero_()
+        run(got, False)
+        assert torch.equal(got, ref)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        run(got, False)
+    for _ in range(8):
+        got.zero_()
+        gr.replay()
+        assert torch.equal(got, ref)
