@@ -96,7 +96,7 @@ template <int STAGES, int SLOTS> struct NarrowCtl {
 template <int BT, int SPLIT>
 __device__ __forceinline__ void join_ranks(const LinParams& P, float4* red, int rank, int m0, int n) {
     constexpr int G = (BT / 4 + SPLIT - 1) / SPLIT;      // groups of four tokens a rank
-    const float b = P.bias ? __ldg(P.bias + n) : 0.f;
+    const float b = P.bias ? P.bias[n] : 0.f;
     float4 v[G][SPLIT];
     #pragma unroll
     for (int g = 0; g < G; g++) {
@@ -218,11 +218,11 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
         float w[G], x[G][PER];
         auto fetch = [&](int kb, float& wv, float (&xv)[PER]) {
             const bool in = kb < kb1;
-            wv = in ? __ldg(wrow + kb) : 0.f;
+            wv = in ? wrow[kb] : 0.f;
             #pragma unroll
             for (int j = 0; j < PER; j++) {
                 const int c = lane + 32 * j;
-                xv[j] = in && c < BT && m0 + c < P.M ? __ldg(P.xs + (size_t)kb * P.M + m0 + c) : 0.f;
+                xv[j] = in && c < BT && m0 + c < P.M ? P.xs[(size_t)kb * P.M + m0 + c] : 0.f;
             }
         };
         #pragma unroll
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(192) k_fp8_linear_narrow(const __grid_constant
     const int nl = (warp & 3) * 32 + lane, n = n0 + nl;
     if (split == 1) {
         if (epi && n < P.N) {
-            const float b = P.bias ? __ldg(P.bias + n) : 0.f;
+            const float b = P.bias ? P.bias[n] : 0.f;
             #pragma unroll
             for (int c = 0; c < BT; c++)
                 if (m0 + c < P.M) store_y(P.y, P.y_type, (size_t)(m0 + c) * P.ldy + n, acc[c] + b);
@@ -621,10 +621,10 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
             bool odd = false;
             if (row < P.M) {
                 const float* p = P.xs + row;
-                #pragma unroll 10
-                for (int kb = 0; kb < P.nkb; kb++) odd |= no_power(__ldg(p + (size_t)kb * P.M));
+                #pragma unroll 20
+                for (int kb = 0; kb < P.nkb; kb++) odd |= no_power(p[(size_t)kb * P.M]);
             }
-            for (int i = threadIdx.x & 127; i < words; i += 128) odd |= no_power(__ldg(P.ws + (size_t)wb0 * P.nkb + i));
+            for (int i = threadIdx.x & 127; i < words; i += 128) odd |= no_power(P.ws[(size_t)wb0 * P.nkb + i]);
             const uint32_t any = __any_sync(0xffffffffu, odd), e = ti % RING;
             if (lane == 0) {
                 // the entry's readers of RING tiles ago are done, in both CTAs
@@ -657,10 +657,10 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
                     #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const int row = m0 + 32 * j + lane;
-                        v.a[j][b] = in && row < P.M ? __ldg(P.xs + (size_t)(kb0 + b) * P.M + row) : 1.f;
+                        v.a[j][b] = in && row < P.M ? P.xs[(size_t)(kb0 + b) * P.M + row] : 1.f;
                     }
                     #pragma unroll
-                    for (int j = 0; j < 3; j++) v.w[j][b] = in && j < wbs ? __ldg(P.ws + (size_t)(wb0 + j) * P.nkb + kb0 + b) : 1.f;
+                    for (int j = 0; j < 3; j++) v.w[j][b] = in && j < wbs ? P.ws[(size_t)(wb0 + j) * P.nkb + kb0 + b] : 1.f;
                 }
                 return v;
             };
@@ -728,9 +728,9 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
                 auto scale = [&](int kb) {
                     Scale v = {0.f, {0.f, 0.f}};
                     if (kb >= P.nkb) return v;
-                    if (px) v.x = __ldg(px + (size_t)kb * P.M);
-                    v.w[0] = n0 / KB < nwb ? __ldg(pw + kb) : 0.f;
-                    v.w[1] = n0 / KB + 1 < nwb ? __ldg(pw + P.nkb + kb) : 0.f;
+                    if (px) v.x = px[(size_t)kb * P.M];
+                    v.w[0] = n0 / KB < nwb ? pw[kb] : 0.f;
+                    v.w[1] = n0 / KB + 1 < nwb ? pw[P.nkb + kb] : 0.f;
                     return v;
                 };
                 Scale v0 = scale(0), v1 = scale(1);
@@ -771,6 +771,8 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
             #pragma unroll
             for (int c = 0; c < C::CH0; c++) {
                 if (c >= nc) break;
+                const int col = n0 + 32 * c;
+                const float bias = P.bias && col + lane < P.N ? P.bias[col + lane] : 0.f;
                 uint32_t d[32];
                 if (way) {
                     sm100::tmem_ld32_async(taddr + (use & 1) * BN + 32 * c, d);
@@ -784,8 +786,6 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
                     #pragma unroll
                     for (int i = 0; i < 16; i++) { d[2 * i] = (uint32_t)acc[c][i]; d[2 * i + 1] = (uint32_t)(acc[c][i] >> 32); }
                 }
-                const int col = n0 + 32 * c;
-                const float bias = P.bias && col + lane < P.N ? __ldg(P.bias + col + lane) : 0.f;
                 // the box's previous store has been read
                 uint8_t* st = box + put * per_box;
                 put = (put + 1) % boxes_n;

@@ -154,8 +154,8 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t m) {
 // 5498 x 6912 (115 MB): 21.7 us, 5.3 TB/s.
 constexpr int QR_ROWS = 32, QR_BLKS = 4;
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256, 3) k_fp8_quant_rows(const T* __restrict__ x, int rows, int cols, int ldx,
-                                                           uint8_t* __restrict__ q, int ldq, float* __restrict__ scale) {
+__global__ void __launch_bounds__(256, 3) k_fp8_quant_rows(const T* x, int rows, int cols, int ldx,
+                                                           uint8_t* q, int ldq, float* scale) {
     constexpr int LANES = 128 / Bits<T>::E, GROUPS = 256 / LANES;
     __shared__ float ss[QR_BLKS][QR_ROWS];
     constexpr bool STAGED = !VEC && sizeof(T) == 2;
@@ -170,27 +170,39 @@ __global__ void __launch_bounds__(256, 3) k_fp8_quant_rows(const T* __restrict__
         if (r0 + i - grp >= rows) break;             // uniform: nothing left for any group
         const long left = r < rows ? cols : 0;
         uint32_t w[QR_BLKS][WORDS];
-        #pragma unroll
-        for (int j = 0; j < QR_BLKS; j++) {
-            if constexpr (!STAGED) {
+        if constexpr (!STAGED) {
+            #pragma unroll
+            for (int j = 0; j < QR_BLKS; j++) {
                 const long c = (b0 + j) * 128L + l * Bits<T>::E;
                 load_lane<T, VEC>(x + (size_t)r * ldx, c, left - c, w[j]);
-            } else {
-                // 16-bit rows that start anywhere: neighbouring lanes load
-                // neighbouring elements of the warp's rows and take their 32 bytes
-                // from shared memory (5498 x 6910: 66 us lane by lane, 33 so; fp32
-                // rows, half as many loads, take 25 us lane by lane and 62 so)
-                T* buf = reinterpret_cast<T*>(sx[threadIdx.x >> 5]);
-                const int lane = threadIdx.x & 31;
-                const long rw = r0 + i - grp + (threadIdx.x >> 5) * (32 / LANES);
+            }
+        } else {
+            // 16-bit rows that start anywhere: neighbouring lanes load neighbouring
+            // elements of the warp's rows, a block ahead, and take their 32 bytes
+            // from shared memory (5498 x 6910: 66 us lane by lane, 33 so; fp32
+            // rows, half as many loads, take 25 us lane by lane and 62 so)
+            constexpr int PER = 32 / LANES * 4;      // a lane's elements of the warp's rows of a block
+            uint4* mine = sx[threadIdx.x >> 5];
+            T* buf = reinterpret_cast<T*>(mine);
+            const int lane = threadIdx.x & 31;
+            const long rw = r0 + i - grp + (threadIdx.x >> 5) * (32 / LANES);
+            T v[PER];
+            auto fetch = [&](int j) {
+                #pragma unroll
+                for (int e = 0; e < PER; e++) {
+                    const long row = rw + e / 4, c = (b0 + j) * 128L + e % 4 * 32 + lane;
+                    v[e] = row < rows && c < cols ? x[(size_t)row * ldx + c] : T(0.f);
+                }
+            };
+            fetch(0);
+            #pragma unroll
+            for (int j = 0; j < QR_BLKS; j++) {
                 __syncwarp();
                 #pragma unroll
-                for (int e = 0; e < 32 / LANES * 4; e++) {
-                    const long row = rw + e / 4, c = (b0 + j) * 128L + e % 4 * 32 + lane;
-                    buf[e * 32 + lane] = row < rows && c < cols ? x[(size_t)row * ldx + c] : T(0.f);
-                }
+                for (int e = 0; e < PER; e++) buf[e * 32 + lane] = v[e];
+                if (j + 1 < QR_BLKS) fetch(j + 1);
                 __syncwarp();
-                const uint4 a = sx[threadIdx.x >> 5][2 * lane], b = sx[threadIdx.x >> 5][2 * lane + 1];
+                const uint4 a = mine[2 * lane], b = mine[2 * lane + 1];
                 w[j][0] = a.x; w[j][1] = a.y; w[j][2] = a.z; w[j][3] = a.w;
                 w[j][4] = b.x; w[j][5] = b.y; w[j][6] = b.z; w[j][7] = b.w;
             }
@@ -218,8 +230,8 @@ __global__ void __launch_bounds__(256, 3) k_fp8_quant_rows(const T* __restrict__
 // Weights: a CTA takes one 128 x 128 block, held in registers between the
 // maximum and the codes.  B200, fp32 7680 x 2560 (98 MB): 20.3 us, 4.8 TB/s.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256, 2) k_fp8_quant_blocks(const T* __restrict__ x, int rows, int cols, int ldx,
-                                                             uint8_t* __restrict__ q, int ldq, float* __restrict__ scale) {
+__global__ void __launch_bounds__(256, 2) k_fp8_quant_blocks(const T* x, int rows, int cols, int ldx,
+                                                             uint8_t* q, int ldq, float* scale) {
     constexpr int LANES = 128 / Bits<T>::E, GROUPS = 256 / LANES, PER = 128 / GROUPS;     // rows a lane
     __shared__ uint32_t sm[8], sf[8];
     chain_begin();

@@ -203,8 +203,8 @@ struct Affine {
     __device__ __forceinline__ void weights(const GnParams& P, int c0) {
         #pragma unroll
         for (int i = 0; i < VEC; i++) {
-            a[i] = P.gamma ? __ldg(P.gamma + c0 + i) : 1.f;
-            beta[i] = P.beta ? __ldg(P.beta + c0 + i) : 0.f;
+            a[i] = P.gamma ? P.gamma[c0 + i] : 1.f;
+            beta[i] = P.beta ? P.beta[c0 + i] : 0.f;
         }
     }
     __device__ __forceinline__ void stats(int i, float4 st) {       // run i

@@ -6,7 +6,9 @@
 // these leave) and waits until the kernels before it have finished and their
 // writes are visible.  A run of them saves the 2 us that a launch after a
 // finished kernel costs; after a kernel that does not take part the wait is
-// over at once.
+// over at once.  What these kernels read was written by others while they were
+// already running, so no load is a read-only one (__ldg, const __restrict__):
+// those promise data that stays the same for the kernel's whole life.
 #pragma once
 #include <cuda_runtime.h>
 
