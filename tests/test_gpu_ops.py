@@ -786,3 +786,22 @@ def test_back_to_back_calls_see_what_the_calls_before_wrote(ctx, T, C, N):
         got.zero_()
         gr.replay()
         assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("t,T,H,D,kw", [
+    (BF16, 60000, 8, 64, dict(axis_dims=[32], layout="half")), (FP32, 60000, 9, 32, dict(axis_dims=[32], layout="half")),
+    (FP16, 80000, 12, 24, dict(axis_dims=[6, 8, 4])), (BF16, 60000, 6, 62, dict(axis_dims=[62])), (BF16, 21000, 6, 33, dict(axis_dims=[32])),
+    (FP32, 3, 2, 4200, dict(axis_dims=[256], layout="half")), (BF16, 3, 2, 4201, dict(axis_dims=[254])),
+])
+def test_rope_many_tokens_and_wide_heads(ctx, t, T, H, D, kw):
+    """CTAs that take several batches of heads, and heads that take several CTAs; into another buffer and in place."""
+    plan = s2b.rope_plan(**kw)
+    x = normal(gen(T + D), 1, T, H, D).to(DT[t])
+    y = torch.full((T * H * D + 64,), 55.0, dtype=DT[t], device=DEV)
+    run_rope(ctx, plan, x, t, None, 0, 7, y[:-64].view(1, T, H, D))
+    pos = (torch.arange(T, device=DEV) + 7)[None, :, None].expand(1, T, plan.axes)
+    ref, mag = rope64(plan, x, pos, False)
+    check_rope(y[:-64].view(1, T, H, D), ref, mag, t, T + 7, plan)
+    assert (y[-64:] == 55).all()
+    run_rope(ctx, plan, x, t, None, 0, 7, x)
+    assert torch.equal(x, y[:-64].view(1, T, H, D))
