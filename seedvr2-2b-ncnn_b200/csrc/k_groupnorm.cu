@@ -4,14 +4,16 @@
 //   mean and (biased) variance over the rows and channels of group g of one
 //   sample.
 //
-// Statistics are fp32: every thread sums d = x - x0 and d^2 about the first
-// value x0 that it meets in a channel, so a mean far from zero cancels
-// nothing, and (n, mean, M2) triples are joined pairwise by
+// Statistics are fp32: a thread takes the values that it holds in registers twice,
+// for their mean and for the deviations from it (on chip), or about the mean so
+// far (streamed, after the first row), and (n, mean, M2) triples are joined
+// pairwise by
 //   mean = m1 + (m2 - m1) n2 / n,  M2 = M2_1 + M2_2 + (m2 - m1)^2 n1 n2 / n
 // (Chan, Golub, LeVeque 1979) in an order that depends on the sizes alone.
-// Means are kept as offsets from the group's first value `ref`, and the
-// normalisation computes (x - ref) - offset: a mean far from zero is never
-// rounded to fp32's step at its own size.
+// A mean is a head and the remainder of its rounding (two-sum, Knuth), and the
+// normalisation computes (x - head) - remainder: a mean far from zero is never
+// rounded to fp32's step at its own size, and nothing hangs on single values:
+// sums about the group's first one lost three digits where that was an outlier.
 //
 // Bound by HBM, or by launches and latency when small.  Two forms:
 //   on chip   a cluster of CTAs takes one sample's slab of whole groups,
@@ -22,13 +24,14 @@
 //             normalisation, which reads x again, last chunk first: what the
 //             statistics read last is still in L2.
 //
-// B200: on chip 1360 x 512 bf16 6.6 us; streamed 3 x 21760 x 512 (134 MB read and
-// written once) 41 us, 1392640 x 128 with SiLU (713 MB, x read twice) 200 us,
-// 184 without: 5.4 TB/s of what DRAM has to move.
+// B200, in a burst: on chip 1360 x 512 bf16 6.4 us; streamed 3 x 21760 x 512 (134 MB
+// read and written once) 38.4 us, 1392640 x 128 with SiLU (713 MB, x read twice)
+// 199 us: 5.4 TB/s of what DRAM has to move.
 #include "kcommon.cuh"
 #include "launch.cuh"
 #include "ops.h"
 #include "sm100.cuh"
+#include <type_traits>
 
 namespace s2b {
 namespace {
@@ -40,8 +43,8 @@ constexpr int CHIP_GROUPS = 64;          // groups of an on-chip slab
 struct GnParams {
     const void* x; void* y;
     const float *gamma, *beta;
-    float4* stat;       // [batch][groups] (ref, mean - ref, rstd, -)
-    float4* part;       // [batch][chunks * tiles][groups] (n, mean - ref, M2, -); n 0: none of the group's channels
+    float4* stat;       // [batch][groups] (mean's head, remainder, rstd, -)
+    float4* part;       // [batch][chunks * tiles][groups] (n, mean's head, remainder, M2); n 0: none of the group's channels
     int rows, C, ldx, ldy, G, cpg;
     int chunk, chunks, tiles;           // streamed
     int slab, slabs, split, share;      // on chip: channels a slab, slabs, CTAs a cluster, rows a CTA
@@ -49,45 +52,91 @@ struct GnParams {
     int silu;
 };
 
-struct Moments { float n, mean, m2; };
+// a + b as the rounded sum and what the rounding lost.
+__device__ __forceinline__ void two_sum(float a, float b, float& head, float& rest) {
+    head = a + b;
+    const float t = head - a;
+    rest = (a - (head - t)) + (b - t);
+}
+
+// n values about the mean hi + lo; M2 is their squared deviations' sum.
+struct Moments { float n, hi, lo, m2; };
+// Without branches: the mean moves from the larger side, by at most half the
+// difference, and an empty side adds nothing.
 __device__ __forceinline__ Moments join(Moments a, Moments b) {
-    if (b.n == 0.f) return a;
-    if (a.n == 0.f) return b;
-    const float n = a.n + b.n, d = b.mean - a.mean, w = __fdividef(b.n, n);
-    return {n, fmaf(d, w, a.mean), a.m2 + b.m2 + d * d * a.n * w};
+    const bool swap = b.n > a.n;
+    const float n = a.n + b.n, few = fminf(a.n, b.n), many = fmaxf(a.n, b.n);
+    const float w = few == 0.f ? 0.f : __fdividef(few, n);
+    float d = (b.hi - a.hi) + (b.lo - a.lo);
+    d = few == 0.f ? 0.f : swap ? -d : d;
+    Moments r = {n, 0.f, 0.f, a.m2 + b.m2 + d * d * many * w};
+    two_sum(swap ? b.hi : a.hi, fmaf(d, w, swap ? b.lo : a.lo), r.hi, r.lo);
+    return r;
 }
 
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Vec { T v[VEC]; };
 
-__device__ __forceinline__ Moments shfl_join(Moments a) {
+// Moments of the `count` values that `each` hands to its argument: about `base`
+// (one of them, so that equal values leave exact zeros) for the mean p, then
+// about p.  base may be any distance off: it only moves p, whose own distance
+// from the mean the second pass makes good.
+template <typename Each>
+__device__ __forceinline__ Moments batch_moments(float count, float inv, float base, Each each) {
+    float s = 0.f, q = 0.f;
+    each([&](float x) { s += x - base; });
+    const float p = fmaf(s, inv, base);
+    s = 0.f;
+    each([&](float x) {
+        const float d = x - p;
+        s += d;
+        q = fmaf(d, d, q);
+    });
+    const float m = s * inv, m2 = fmaf(-s, m, q);
+    Moments r = {count, 0.f, 0.f, m2 < 0.f ? 0.f : m2};          // NaN stays
+    two_sum(p, m, r.hi, r.lo);
+    return r;
+}
+
+// Joined over each `lanes` (a power of two) neighbouring lanes, into their first.
+__device__ __forceinline__ Moments shfl_join(Moments a, int lanes) {
     #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
-        a = join(a, {__shfl_down_sync(0xffffffffu, a.n, o), __shfl_down_sync(0xffffffffu, a.mean, o),
-                     __shfl_down_sync(0xffffffffu, a.m2, o)});
+        if (o < lanes)
+            a = join(a, {__shfl_down_sync(0xffffffffu, a.n, o), __shfl_down_sync(0xffffffffu, a.hi, o),
+                         __shfl_down_sync(0xffffffffu, a.lo, o), __shfl_down_sync(0xffffffffu, a.m2, o)});
     return a;
 }
 
-// Joins what the threads of a CTA hold of each group: sm[k * width + c] is
-// (mean - ref, M2) of row lane k and the CTA's run c of SUB channels (the
-// first is the operator's run c0), from count(k) rows of them.  One warp a
-// group, lanes over its runs and row lanes; done(g, moments) runs on lane 0.
+// Joins what the threads of a CTA hold of each group: sm[k * width + c] is the
+// mean and M2 of row lane k and the CTA's run c of SUB channels (the first is
+// the operator's run c0), from count(k) rows of them.  As many threads a group,
+// up to a warp, as make one round of it, over its runs and row lanes (a warp a
+// group, four rounds of six joins for 32 groups: 43.4 us against 38.4 for three
+// samples of 21760 x 512); done(g, moments) runs on the first.
 template <int SUB, typename Count, typename Done>
-__device__ __forceinline__ void join_groups(const float2* sm, int width, int lanes, int c0, int cpg, Count count, Done done) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = cpg / SUB;     // runs a group
-    const int g0 = c0 / per, g1 = (c0 + width - 1) / per;
-    for (int g = g0 + warp; g <= g1; g += THREADS / 32) {
-        const int a = max(g * per - c0, 0), b = min((g + 1) * per - c0, width), w = b - a;
-        Moments m = {0.f, 0.f, 0.f};
-        int k = lane / w, c = lane - k * w;
-        const int dk = 32 / w, dc = 32 - dk * w;
+__device__ __forceinline__ void join_groups(const float3* sm, int width, int lanes, int c0, int cpg, Count count, Done done) {
+    const int per = cpg / SUB;                   // runs a group
+    const int g0 = c0 / per, groups = (c0 + width - 1) / per - g0 + 1;
+    int lg = 5;
+    while (lg > 0 && groups << lg > THREADS) lg--;
+    const int L = 1 << lg, l = threadIdx.x & (L - 1);
+    for (int first = 0; first < groups; first += THREADS >> lg) {
+        const int g = g0 + first + (threadIdx.x >> lg);
+        if (!__any_sync(0xffffffffu, g < g0 + groups)) break;
+        const bool on = g < g0 + groups;
+        const int a = max(g * per - c0, 0), w = on ? min((g + 1) * per - c0, width) - a : 1;
+        Moments m = {0.f, 0.f, 0.f, 0.f};
+        int k = on ? l / w : lanes, c = l - l / w * w;
+        const int dk = L / w, dc = L - dk * w;
         for (; k < lanes;) {
-            const float2 v = sm[k * width + a + c];
-            m = join(m, {(float)(count(k) * SUB), v.x, v.y});
+            const float3 v = sm[k * width + a + c];
+            m = join(m, {(float)(count(k) * SUB), v.x, v.y, v.z});
             k += dk; c += dc;
             if (c >= w) { c -= w; k++; }
         }
-        m = shfl_join(m);
-        if (lane == 0) done(g, m);
+        __syncwarp();
+        m = shfl_join(m, L);
+        if (on && l == 0) done(g, m);
     }
 }
 
@@ -100,53 +149,89 @@ template <typename T, int VEC, int SUB>
 __global__ void __launch_bounds__(THREADS, STATS_CTAS) k_gn_stats(const GnParams P) {
     typedef Vec<T, VEC> V;
     constexpr int N = VEC / SUB, UNROLL = 8;
-    __shared__ float2 sm[THREADS * N];
+    __shared__ float3 sm[THREADS * N];
     chain_begin();
     const int vecs = P.C / VEC, tw = tile_cols(vecs), rp = THREADS / tw;
     const int tc = threadIdx.x % tw, tr = threadIdx.x / tw;
     const int vc = blockIdx.y * tw + tc;
     const int r0 = blockIdx.x * P.chunk, r1 = min(P.rows, r0 + P.chunk);
     const bool on = tr < rp && vc < vecs;
-    const T* base = (const T*)P.x + ((size_t)blockIdx.z * P.rows) * P.ldx;
-    const T* x = base + (size_t)vc * VEC;
-    float x0[N], s[N], q[N];
+    const T* x = (const T*)P.x + ((size_t)blockIdx.z * P.rows) * P.ldx + (size_t)vc * VEC;
+    // n values so far about the mean hi + lo, and their M2, run by run
+    float n = 0.f, hi[N], lo[N], m2[N];
     #pragma unroll
-    for (int i = 0; i < N; i++) { x0[i] = 0.f; s[i] = 0.f; q[i] = 0.f; }
-    auto add = [&](const V& u) {
-        #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const float d = Cvt<T>::to_f(u.v[i]) - x0[i / SUB];
-            s[i / SUB] += d;
-            q[i / SUB] = fmaf(d, d, q[i / SUB]);
-        }
-    };
-    const int width = (min(tw * VEC, P.C - (int)blockIdx.y * tw * VEC)) / SUB, len = r1 - r0;
-    if (on) {
-        int n = 0;
-        if (r0 + tr < r1) {
-            const V f = *reinterpret_cast<const V*>(x + (size_t)(r0 + tr) * P.ldx);
-            #pragma unroll
-            for (int i = 0; i < N; i++) x0[i] = Cvt<T>::to_f(f.v[i * SUB]);
-            n = (len - tr + rp - 1) / rp;
-            const T* p = x + (size_t)(r0 + tr) * P.ldx;
-            const size_t step = (size_t)rp * P.ldx;
-            int k = 0;
-            for (; k + UNROLL <= n; k += UNROLL, p += UNROLL * step) {
-                V u[UNROLL];
-                #pragma unroll
-                for (int j = 0; j < UNROLL; j++) u[j] = *reinterpret_cast<const V*>(p + j * step);
-                #pragma unroll
-                for (int j = 0; j < UNROLL; j++) add(u[j]);
-            }
-            for (; k < n; k++, p += step) add(*reinterpret_cast<const V*>(p));
-        }
-        const float inv = n ? 1.f / (float)(n * SUB) : 0.f;
+    for (int i = 0; i < N; i++) { hi[i] = 0.f; lo[i] = 0.f; m2[i] = 0.f; }
+    auto first = [&](const V& u) {
+        n = SUB;
         #pragma unroll
         for (int i = 0; i < N; i++) {
-            const float m = s[i] * inv, m2 = q[i] - s[i] * m;
-            const float ref = Cvt<T>::to_f(base[(vc * VEC + i * SUB) / P.cpg * P.cpg]);
-            sm[tr * width + tc * N + i] = make_float2((x0[i] - ref) + m, m2 < 0.f ? 0.f : m2);     // NaN stays
+            const Moments m = batch_moments(SUB, 1.f / SUB, Cvt<T>::to_f(u.v[i * SUB]), [&](auto take) {
+                #pragma unroll
+                for (int c = 0; c < SUB; c++) take(Cvt<T>::to_f(u.v[i * SUB + c]));
+            });
+            hi[i] = m.hi; lo[i] = m.lo; m2[i] = m.m2;
         }
+    };
+    // Rows J .. of u: B values of a run.  With s, q the sums of e = x - mean and of
+    // e^2, M2 grows by q - s^2 / (n + B) >= q n / (n + B): an eighth of q behind the
+    // first row, half or more from then on, so little cancels wherever the values
+    // lie.  (Two passes over every batch took 10 to 15 % longer where groups cut
+    // vectors.)
+    auto more = [&](const auto& u, auto from) {
+        constexpr int J = decltype(from)::value, R = sizeof(u) / sizeof(V), B = (R - J) * SUB;
+        n += B;
+        const float inv = __fdividef(1.f, n);
+        #pragma unroll
+        for (int i = 0; i < N; i++) {
+            float s = 0.f, q = 0.f;
+            #pragma unroll
+            for (int j = J; j < R; j++)
+                #pragma unroll
+                for (int c = 0; c < SUB; c++) {
+                    const float d = Cvt<T>::to_f(u[j].v[i * SUB + c]) - hi[i];
+                    s += d;
+                    q = fmaf(d, d, q);
+                }
+            const float t = fmaf(-(float)B, lo[i], s);           // about the remainder too
+            q = fmaf(-lo[i], s + t, q);
+            m2[i] += fmaf(-t * inv, t, q);
+            // fast two-sum (Dekker): where the mean moves by more than its own
+            // size it errs by a rounding of the step, which M2 holds
+            const float g = fmaf(t, inv, lo[i]), h = hi[i] + g;
+            lo[i] = g - (h - hi[i]);
+            hi[i] = h;
+        }
+    };
+    const std::integral_constant<int, 0> whole;
+    const std::integral_constant<int, 1> rest;
+    const int width = (min(tw * VEC, P.C - (int)blockIdx.y * tw * VEC)) / SUB, len = r1 - r0;
+    if (on) {
+        if (r0 + tr < r1) {
+            const int rows = (len - tr + rp - 1) / rp;
+            const T* p = x + (size_t)(r0 + tr) * P.ldx;
+            const size_t step = (size_t)rp * P.ldx;
+            auto load = [&](auto& u) {
+                constexpr int R = sizeof(u) / sizeof(V);
+                #pragma unroll
+                for (int j = 0; j < R; j++) u[j] = *reinterpret_cast<const V*>(p + j * step);
+                p += R * step;
+            };
+            V u[UNROLL], one[1];
+            int k = 0;
+            if (rows >= UNROLL) {
+                load(u);
+                first(u[0]);
+                more(u, rest);
+                for (k = UNROLL; k + UNROLL <= rows; k += UNROLL) { load(u); more(u, whole); }
+            } else {
+                load(one);
+                first(one[0]);
+                k = 1;
+            }
+            for (; k < rows; k++) { load(one); more(one, whole); }
+        }
+        #pragma unroll
+        for (int i = 0; i < N; i++) sm[tr * width + tc * N + i] = make_float3(hi[i], lo[i], m2[i] < 0.f ? 0.f : m2[i]);     // NaN stays
     }
     // groups that have no channel in this tile
     float4* part = P.part + (((size_t)blockIdx.z * P.chunks + blockIdx.x) * P.tiles + blockIdx.y) * P.G;
@@ -158,37 +243,36 @@ __global__ void __launch_bounds__(THREADS, STATS_CTAS) k_gn_stats(const GnParams
     }
     __syncthreads();
     join_groups<SUB>(sm, width, rp, run0, P.cpg, [&](int k) { return k < len ? (len - k + rp - 1) / rp : 0; },
-                     [&](int g, Moments m) { part[g] = make_float4(m.n, m.mean, m.m2, 0.f); });
+                     [&](int g, Moments m) { part[g] = make_float4(m.n, m.hi, m.lo, m.m2); });
 }
 
-__device__ __forceinline__ float4 finish(float ref, Moments m, float eps) {
-    return make_float4(ref, m.mean, 1.f / sqrtf(m.m2 / m.n + eps), 0.f);
+__device__ __forceinline__ float4 finish(Moments m, float eps) {
+    return make_float4(m.hi, m.lo, 1.f / sqrtf(m.m2 / m.n + eps), 0.f);
 }
 
 // One CTA joins the chunks of one group of one sample: at most four of them a
 // thread at the usual sizes, all loaded together.
-template <typename T>
 __global__ void __launch_bounds__(128) k_gn_join(const GnParams P) {
     __shared__ float4 sm[4];
     chain_begin();
     const int g = blockIdx.x, b = blockIdx.y;
-    const float ref = Cvt<T>::to_f(((const T*)P.x)[(size_t)b * P.rows * P.ldx + (size_t)g * P.cpg]);
     const int entries = P.chunks * P.tiles;
     const float4* part = P.part + (size_t)b * entries * P.G + g;
-    Moments a = {0.f, 0.f, 0.f};
+    Moments a = {0.f, 0.f, 0.f, 0.f};
     for (int e = threadIdx.x; e < entries; e += 4 * 128) {
         float4 v[4];
         #pragma unroll
         for (int k = 0; k < 4; k++) v[k] = e + 128 * k < entries ? part[(size_t)(e + 128 * k) * P.G] : make_float4(0.f, 0.f, 0.f, 0.f);
-        #pragma unroll
-        for (int k = 0; k < 4; k++) a = join(a, {v[k].x, v[k].y, v[k].z});
+        const auto of = [](float4 f) { return Moments{f.x, f.y, f.z, f.w}; };
+        const Moments four = join(join(of(v[0]), of(v[1])), join(of(v[2]), of(v[3])));
+        a = e == (int)threadIdx.x ? four : join(a, four);
     }
-    a = shfl_join(a);
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = make_float4(a.n, a.mean, a.m2, 0.f);
+    a = shfl_join(a, 32);
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = make_float4(a.n, a.hi, a.lo, a.m2);
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < 4; i++) a = join(a, {sm[i].x, sm[i].y, sm[i].z});
-        P.stat[(size_t)b * P.G + g] = finish(ref, a, P.eps);
+        const auto at = [&](int i) { return Moments{sm[i].x, sm[i].y, sm[i].z, sm[i].w}; };
+        P.stat[(size_t)b * P.G + g] = finish(join(join(a, at(1)), join(at(2), at(3))), P.eps);
     }
 }
 
@@ -196,10 +280,10 @@ __global__ void __launch_bounds__(128) k_gn_join(const GnParams P) {
 // far below a 16-bit output's half step and within a few steps of fp32's.
 __device__ __forceinline__ float gn_silu(float v) { return v * __fdividef(1.f, 1.f + __expf(-v)); }
 
-// act((x - ref - mean) * a + beta) of VEC channels.
+// act(((x - hi) - lo) * a + beta) of VEC channels.
 template <typename TX, typename TY, int VEC, int SUB>
 struct Affine {
-    float ref[VEC / SUB], mean[VEC / SUB], a[VEC], beta[VEC];
+    float hi[VEC / SUB], lo[VEC / SUB], a[VEC], beta[VEC];
     __device__ __forceinline__ void weights(const GnParams& P, int c0) {
         #pragma unroll
         for (int i = 0; i < VEC; i++) {
@@ -208,8 +292,8 @@ struct Affine {
         }
     }
     __device__ __forceinline__ void stats(int i, float4 st) {       // run i
-        ref[i] = st.x;
-        mean[i] = st.y;
+        hi[i] = st.x;
+        lo[i] = st.y;
         #pragma unroll
         for (int j = i * SUB; j < (i + 1) * SUB; j++) a[j] *= st.z;
     }
@@ -218,7 +302,7 @@ struct Affine {
         Vec<TY, VEC> o;
         #pragma unroll
         for (int i = 0; i < VEC; i++) {
-            float v = fmaf((Cvt<TX>::to_f(u.v[i]) - ref[i / SUB]) - mean[i / SUB], a[i], beta[i]);
+            float v = fmaf((Cvt<TX>::to_f(u.v[i]) - hi[i / SUB]) - lo[i / SUB], a[i], beta[i]);
             if (SILU) v = gn_silu(v);
             o.v[i] = Cvt<TY>::from_f(v);
         }
@@ -275,10 +359,9 @@ __global__ void __launch_bounds__(THREADS, RV <= 4 ? 3 : 2) k_gn_chip(const GnPa
     typedef Vec<TX, VEC> VX;
     typedef Vec<TY, VEC> VY;
     constexpr int N = VEC / SUB;
-    __shared__ float2 sm[THREADS * N];
-    __shared__ float4 mine[CHIP_GROUPS];         // this CTA's (n, mean - ref, M2) of the slab's groups
+    __shared__ float3 sm[THREADS * N];
+    __shared__ float4 mine[CHIP_GROUPS];         // this CTA's moments of the slab's groups
     __shared__ float4 stat[CHIP_GROUPS];
-    __shared__ float sref[CHIP_GROUPS];
     chain_begin();
     const int rank = P.split > 1 ? (int)sm100::cluster_ctarank() : 0;
     const int item = blockIdx.x / P.split, b = item / P.slabs, c0 = item % P.slabs * P.slab;
@@ -291,7 +374,6 @@ __global__ void __launch_bounds__(THREADS, RV <= 4 ? 3 : 2) k_gn_chip(const GnPa
     const int groups = P.slab / P.cpg;
     VX u[RV];
     Affine<TX, TY, VEC, SUB> f;
-    if (threadIdx.x < groups) sref[threadIdx.x] = Cvt<TX>::to_f(base[threadIdx.x * P.cpg]);
     if (on) {
         f.weights(P, c0 + tc * VEC);
         const TX* p = base + (size_t)(r0 + tr) * P.ldx + tc * VEC;
@@ -299,36 +381,25 @@ __global__ void __launch_bounds__(THREADS, RV <= 4 ? 3 : 2) k_gn_chip(const GnPa
         #pragma unroll
         for (int k = 0; k < RV; k++)
             if (k < n) u[k] = *reinterpret_cast<const VX*>(p + k * step);
-        float ref[N];
+        const float count = (float)(n * SUB), inv = n ? 1.f / count : 0.f;
         #pragma unroll
-        for (int i = 0; i < N; i++) ref[i] = Cvt<TX>::to_f(base[(tc * VEC + i * SUB) / P.cpg * P.cpg]);
-        float s[N], q[N];
-        #pragma unroll
-        for (int i = 0; i < N; i++) s[i] = q[i] = 0.f;
-        #pragma unroll
-        for (int k = 0; k < RV; k++)
-            if (k < n) {
-                #pragma unroll
-                for (int i = 0; i < VEC; i++) s[i / SUB] += Cvt<TX>::to_f(u[k].v[i]) - ref[i / SUB];
-            }
-        const float inv = n ? 1.f / (float)(n * SUB) : 0.f;
-        #pragma unroll
-        for (int i = 0; i < N; i++) s[i] *= inv;
-        #pragma unroll
-        for (int k = 0; k < RV; k++)
-            if (k < n) {
-                #pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    const float d = (Cvt<TX>::to_f(u[k].v[i]) - ref[i / SUB]) - s[i / SUB];
-                    q[i / SUB] = fmaf(d, d, q[i / SUB]);
-                }
-            }
-        #pragma unroll
-        for (int i = 0; i < N; i++) sm[tr * width + tc * N + i] = make_float2(s[i], q[i]);
+        for (int i = 0; i < N; i++) {
+            Moments m = {0.f, 0.f, 0.f, 0.f};
+            if (n)
+                m = batch_moments(count, inv, Cvt<TX>::to_f(u[0].v[i * SUB]), [&](auto take) {
+                    #pragma unroll
+                    for (int k = 0; k < RV; k++)
+                        if (k < n) {
+                            #pragma unroll
+                            for (int c = 0; c < SUB; c++) take(Cvt<TX>::to_f(u[k].v[i * SUB + c]));
+                        }
+                });
+            sm[tr * width + tc * N + i] = make_float3(m.hi, m.lo, m.m2);
+        }
     }
     __syncthreads();
     join_groups<SUB>(sm, width, rp, 0, P.cpg, [&](int k) { return k < len ? (len - k + rp - 1) / rp : 0; },
-                     [&](int g, Moments m) { mine[g] = make_float4(m.n, m.mean, m.m2, 0.f); });
+                     [&](int g, Moments m) { mine[g] = make_float4(m.n, m.hi, m.lo, m.m2); });
     if (P.split > 1) sm100::cluster_sync();
     else __syncthreads();
     // a warp a group, a lane a rank: the ranks' moments arrive together
@@ -336,11 +407,10 @@ __global__ void __launch_bounds__(THREADS, RV <= 4 ? 3 : 2) k_gn_chip(const GnPa
         const int r = threadIdx.x & 31;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r < P.split) v = P.split > 1 ? sm100::ld_cluster_f32x4(sm100::map_to_rank(&mine[g], r)) : mine[g];
-        const Moments a = shfl_join({v.x, v.y, v.z});
-        if (r == 0) stat[g] = finish(sref[g], a, P.eps);
+        const Moments a = shfl_join({v.x, v.y, v.z, v.w}, 8);      // up to eight ranks
+        if (r == 0) stat[g] = finish(a, P.eps);
     }
-    // every rank has read the others' moments and row 0's references: shared
-    // memory may go away and y (which may be x) may be written
+    // every rank has read the others' moments: shared memory may go away
     if (P.split > 1) sm100::cluster_sync();
     else __syncthreads();
     if (!on) return;
@@ -411,7 +481,7 @@ int launch_v(const GroupNormArgs& a, GnParams& P, cudaStream_t s) {
     P.part = P.stat + (size_t)a.batch * P.G;
     const dim3 g(P.chunks, P.tiles, a.batch), ga((a.rows + achunk - 1) / achunk, P.tiles, a.batch);
     if (!launch_chained(k_gn_stats<TX, VEC, SUB>, g, THREADS, 0, 0, s, P)) return -1;
-    if (!launch_chained(k_gn_join<TX>, dim3(P.G, a.batch), 128, 0, 0, s, P)) return -1;
+    if (!launch_chained(k_gn_join, dim3(P.G, a.batch), 128, 0, 0, s, P)) return -1;
     if (!launch_chained(k_gn_apply<TX, TY, VEC, SUB>, ga, THREADS, 0, 0, s, P)) return -1;
     return 3;
 }

@@ -522,6 +522,37 @@ def test_groupnorm_nan_and_inf_stay_in_their_group(ctx):
     assert torch.equal(y, ref)
 
 
+def unlike_first_values(kind, size, B, S, C, G, t):
+    """Inputs whose groups begin with values unlike the rest."""
+    g = gen(S + C + G)
+    x = normal(g, B, S, C)
+    if kind == "first":                    # one value: the group's first
+        x[:, 0, :: C // G] = size
+    elif kind == "head":                   # the first rows, which many threads begin with
+        x[:, : max(1, min(64, S // 4))] *= size
+    elif kind == "padding":                # rows of zeros ahead of far values
+        x += size
+        x[:, : max(1, S // 16)] = 0
+    else:                                  # a lone value in zeros
+        x.zero_()
+        x[:, 0, :: C // G] = size
+    return x.to(DT[t])
+
+
+@pytest.mark.parametrize("kind", ["first", "head", "padding", "lone"])
+@pytest.mark.parametrize("B,S,C,G", [(2, 300, 64, 8), (1, 300, 64, 64), (1, 7000, 64, 16), (2, 40000, 64, 8), (1, 40000, 64, 64), (1, 21760, 128, 32),
+                                     (1, 30000, 60, 4), (1, 300, 10, 1), (1, 200000, 10, 2), (1, 40003, 64, 1)])
+def test_groupnorm_first_values_unlike_the_rest(ctx, B, S, C, G, kind):
+    """No value of a group is special: one that lies 30 to 300000 deviations off the rest, where the group begins or in
+    every thread's first rows, costs no accuracy anywhere.  Deviations are differences to a batch's own mean (rounded
+    relative to themselves), their squares sum to what the group's M2 holds, and means move by a share of a difference
+    that M2 holds too: the roundings of check_norm, counted against the group's spread, are all there are."""
+    for xt in (FP32, BF16):
+        for size in (30.0, 1000.0, 4097.0, 300000.0):
+            x = unlike_first_values(kind, size, B, S, C, G, xt)
+            check_norm(run_norm(ctx, x, G, None, None, 1e-6, False, FP32), x, G, None, None, 1e-6, False, FP32)
+
+
 @pytest.mark.parametrize("C,pad,off", [(64, 8, 0), (64, 3, 0), (60, 0, 2), (512, 16, 8)])
 @pytest.mark.parametrize("t", [FP32, BF16], ids=IDS)
 def test_groupnorm_pitches_in_place_and_unaligned(ctx, t, C, pad, off):
