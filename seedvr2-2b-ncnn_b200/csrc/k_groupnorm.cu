@@ -26,7 +26,7 @@
 //
 // B200, in a burst: on chip 1360 x 512 bf16 6.4 us; streamed 3 x 21760 x 512 (134 MB
 // read and written once) 38.4 us, 1392640 x 128 with SiLU (713 MB, x read twice)
-// 199 us: 5.4 TB/s of what DRAM has to move.
+// 197 us: 5.4 TB/s of what DRAM has to move.
 #include "kcommon.cuh"
 #include "launch.cuh"
 #include "ops.h"
@@ -276,9 +276,23 @@ __global__ void __launch_bounds__(128) k_gn_join(const GnParams P) {
     }
 }
 
-// v / (1 + e^-v); the fast exponential and division are off by 2^-21 together,
-// far below a 16-bit output's half step and within a few steps of fp32's.
-__device__ __forceinline__ float gn_silu(float v) { return v * __fdividef(1.f, 1.f + __expf(-v)); }
+// v sigmoid(v) = v / (1 + e^-v), from e^-|v| so that nothing overflows and the
+// denominator lies in [1, 2].  fp32 outputs take expf, within 2 ulp.  For 16-bit
+// ones e^-|v| is the square of 2^(-|v| log2(e) / 2): the instruction's flush of
+// subnormal results is out of reach, the square may be subnormal, and the error,
+// |v| + 5 ulp of fp32, is far below their half step.
+template <typename TY>
+__device__ __forceinline__ float gn_silu(float v) {
+    float e, r;
+    if (sizeof(TY) == 4) {
+        e = expf(-fabsf(v));
+        return __fdividef(v < 0.f ? v * e : v, 1.f + e);
+    }
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fabsf(v) * -0.72134752f));
+    e *= e;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return (v < 0.f ? v * e : v) * r;
+}
 
 // act(((x - hi) - lo) * a + beta) of VEC channels.
 template <typename TX, typename TY, int VEC, int SUB>
@@ -303,7 +317,7 @@ struct Affine {
         #pragma unroll
         for (int i = 0; i < VEC; i++) {
             float v = fmaf((Cvt<TX>::to_f(u.v[i]) - hi[i / SUB]) - lo[i / SUB], a[i], beta[i]);
-            if (SILU) v = gn_silu(v);
+            if (SILU) v = gn_silu<TY>(v);
             o.v[i] = Cvt<TY>::from_f(v);
         }
         return o;

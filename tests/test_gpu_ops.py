@@ -511,6 +511,24 @@ def test_groupnorm_far_means_and_flat_groups(ctx):
     assert torch.equal(y, beta.expand(1, 500, 32))
 
 
+@pytest.mark.parametrize("S", [40, 40000])
+@pytest.mark.parametrize("t", [FP32, FP16, BF16], ids=IDS)
+def test_groupnorm_silu_over_its_whole_range(ctx, t, S):
+    """Constant groups, so that y = beta * sigmoid(beta) of known betas: from where the exponential leaves fp32's range to
+    where it is 1.  fp32: the exponential errs by 2 ulp, the sum in the denominator by a rounding, its quotient by 2 ulp,
+    the product by a rounding: 10 * 2^-24; for 16-bit outputs the fast exponential errs by |beta| + 5 ulp, the rest by 2
+    more, next to their own half step.  Exponentials below 2^-126 are held to a few steps of 2^-149."""
+    C = 512
+    beta = torch.linspace(-120.0, 30.0, C, device=DEV)
+    x = torch.full((1, S, C), 2.5, device=DEV, dtype=DT[t])
+    y = run_norm(ctx, x, 4, None, beta, 1e-6, True, t)
+    ref = (beta.double() * torch.sigmoid(beta.double()))[None, None]
+    units = 10 if t == FP32 else 2 * (7 + beta.abs().double())
+    tol = (1.01 * units * 2.0 ** -24 + (0 if t == FP32 else HALF[t])) * ref.abs() + 3 * 2.0 ** -149 * beta.abs().double() + TINY[t]
+    err = (y.double() - ref).abs()
+    assert (err <= tol).all(), ((err / tol).max().item(), beta[(err / tol).amax(dim=(0, 1)).argmax()].item())
+
+
 def test_groupnorm_nan_and_inf_stay_in_their_group(ctx):
     g = gen(12)
     x = normal(g, 2, 900, 64)
