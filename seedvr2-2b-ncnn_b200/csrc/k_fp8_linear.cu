@@ -35,9 +35,11 @@ struct LinParams {
 };
 
 // Bounded wait; on expiry raises the CTA's abort flag and the device flag.
+// CLUSTER: on a barrier that the other CTA of a pair arrives at.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait_flag(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* flag) {
     for (uint32_t i = 0; i < sm100::WAIT_LIMIT; i++) {
-        if (sm100::mbar_try_wait(bar, parity)) return true;
+        if (CLUSTER ? sm100::mbar_try_wait_cluster(bar, parity) : sm100::mbar_try_wait(bar, parity)) return true;
         if ((i & 1023) == 1023 && *abort_flag) return false;
     }
     *abort_flag = 1;
@@ -47,9 +49,10 @@ __device__ __forceinline__ bool wait_flag(uint64_t* bar, uint32_t parity, volati
 
 // The same for waits of thousands of cycles: the warp sleeps between polls and
 // leaves the issue slots of its scheduler to the warps that feed the tensor core.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool wait_flag_idle(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* flag) {
     for (uint32_t i = 0; i < (1u << 22); i++) {
-        if (sm100::mbar_try_wait(bar, parity)) return true;
+        if (CLUSTER ? sm100::mbar_try_wait_cluster(bar, parity) : sm100::mbar_try_wait(bar, parity)) return true;
         if ((i & 255) == 255 && *abort_flag) return false;
         __nanosleep(100);
     }
@@ -337,15 +340,16 @@ int launch_narrow(const Fp8LinearArgs& a, const LinParams& P, cudaStream_t s) {
 //
 // The general way is bound by the round trip MMA -> commit -> TMEM read ->
 // release -> MMA, about 2700 cycles for two blocks of 470 (5498 x 2560 x 13824:
-// 344 us).  The scaled one takes about 610 cycles a block where the MMAs alone
+// 360 us in a burst, where a form of this kernel without the scaled way, its
+// accumulators read 32 columns at a time, took 226). The scaled one takes about 610 cycles a block where the MMAs alone
 // need 470 (shared memory feeds the tensor core and takes the loads at the same
-// time) and loses 10 % between tiles: 178 us, 2.2 PFLOP/s; in a long run the
-// 1000 W cap lowers the clock and it takes 214 us.
+// time) and loses 10 % between tiles: 173 us, 2.2 PFLOP/s; in a long run the
+// 1000 W cap lowers the clock and it takes a fifth longer.
 //
 // Warpgroup 0: warps 0 and 2 load by TMA, warp 1 (even CTA) issues the MMAs.
-// Warpgroup 1 looks at each tile's scales, a tile ahead or more, agrees with the
-// other CTA's on the way, and writes the scale bytes of four blocks at a
-// time to TMEM.  Warpgroups 2 and 3 are the epilogue: a warp owns 32 rows and
+// Warpgroup 1 looks at its CTA's part of each tile's scales, a tile ahead, tells
+// both CTAs, and writes the scale bytes of four blocks at a time to TMEM; warp 3
+// passes on that a verdict's readers are done.  Warpgroups 2 and 3 are the epilogue: a warp owns 32 rows and
 // CH0 (the rest) chunks of 32 columns -- a chunk lies in one weight block.
 // Two consecutive blocks share one full barrier (a wait costs the MMA warp about
 // 200 cycles), each stage has its own done barrier (loads follow one by one).
@@ -366,7 +370,8 @@ template <int BN> struct PairCfg8 {
 struct alignas(16) PairCtl {
     uint64_t full[PBARS], done[PSTAGES], tfull[2], tempty[2];
     uint64_t sfull[RING], sempty[RING];          // scale bytes of four blocks
-    uint64_t mfull[RING], mempty[RING];          // the way a tile runs
+    uint64_t mfull[RING], mempty[RING];          // the way a tile runs; this CTA's readers of it are done
+    uint64_t mgone[RING];                        // both CTAs' are
     uint4 odd[RING][2];                          // word q of CTA r: a scale that its warp q looked at is no power of two
     uint32_t tmem_slot;
     int abort;
@@ -472,8 +477,9 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
         for (int i = 0; i < RING; i++) {
             sm100::mbar_init(&ctl->sfull[i], 8);         // warpgroup 1 of both CTAs
             sm100::mbar_init(&ctl->sempty[i], 1);
-            sm100::mbar_init(&ctl->mfull[i], 8);         // the same
-            sm100::mbar_init(&ctl->mempty[i], 25);       // 12 reading warps of each CTA and the MMA warp
+            sm100::mbar_init(&ctl->mfull[i], 5);         // this CTA's, and the expectation of the other's four words
+            sm100::mbar_init(&ctl->mempty[i], rank == 0 ? 13 : 12);      // warpgroups 1 to 3, the MMA warp
+            sm100::mbar_init(&ctl->mgone[i], 2);         // warp 3 of both CTAs
         }
         ctl->abort = 0;
         sm100::fence_barrier_init();
@@ -509,7 +515,7 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
         const uint4 a = ctl->odd[e][0], b = ctl->odd[e][1];
         const int way = !(a.x | a.y | a.z | a.w | b.x | b.y | b.z | b.w);
         __syncwarp();
-        if (lane < 2) sm100::mbar_arrive_cluster_cta(sm100::map_to_rank(&ctl->mempty[e], lane));
+        if (lane == 0) sm100::mbar_arrive(&ctl->mempty[e]);
         return way;
     };
 
@@ -545,6 +551,14 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
                     const long k = issued - i;
                     for (uint32_t w = 0; w < sm100::WAIT_LIMIT && !sm100::mbar_try_wait(&ctl->full[k % PBARS], (k / PBARS) & 1); w++) {}
                 }
+        } else if (warp == 3 && lane == 0) {
+            // the release to the cluster that no reader of a verdict waits for
+            uint32_t ti = 0;
+            for (int tile = pair; tile < T.total; tile += npairs, ti++) {
+                const uint32_t e = ti % RING;
+                if (!wait_flag_idle(&ctl->mempty[e], (ti / RING) & 1, abort_flag, P.flag)) break;
+                for (uint32_t r = 0; r < 2; r++) sm100::mbar_arrive_cluster(sm100::map_to_rank(&ctl->mgone[e], r));
+            }
         } else if (warp == 1 && rank == 0) {
             constexpr uint32_t idesc = sm100::idesc_e4m3_f32(PBM, BN);
             const uint64_t da = sm100::desc_kmajor_sw128(smem, 0), db = sm100::desc_kmajor_sw128(smem + C::A_TILE, 0);
@@ -553,14 +567,15 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
             uint32_t ph = 0, use = 0, grp = 0, ti = 0;     // stage, slot uses, groups of scale bytes, tiles
             bool ok = true;
             auto wait = [&](uint64_t* bar, uint32_t par) { return __all_sync(0xffffffffu, wait_flag(bar, par, abort_flag, P.flag)) != 0; };
+            auto wait_cluster = [&](uint64_t* bar, uint32_t par) { return __all_sync(0xffffffffu, wait_flag<true>(bar, par, abort_flag, P.flag)) != 0; };
             for (int tile = pair; tile < T.total && ok; tile += npairs, ti++) {
                 const int way = tile_way(ti);
                 if (way < 0) break;
                 if (way) {
                     const uint32_t slot = use & 1, d = tmem + slot * BN;
-                    if (!(ok = wait(&ctl->tempty[slot], ((use >> 1) & 1) ^ 1))) break;
+                    if (!(ok = wait_cluster(&ctl->tempty[slot], ((use >> 1) & 1) ^ 1))) break;
                     for (int kb0 = 0; kb0 < P.nkb && ok; kb0 += 4, grp++) {
-                        if (!(ok = wait(&ctl->sfull[grp % RING], (grp / RING) & 1))) break;
+                        if (!(ok = wait_cluster(&ctl->sfull[grp % RING], (grp / RING) & 1))) break;
                         const uint32_t sf = tmem + C::SF + grp % RING * 16;
                         #pragma unroll
                         for (int h = 0; h < 2; h++) {
@@ -594,7 +609,7 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
                     for (int kb = 0; kb < P.nkb; kb++, use++) {
                         const uint32_t slot = use & 1, d = tmem + slot * BN;
                         if (!(kb & 1) && !(ok = wait(&ctl->full[s], ph))) break;
-                        if (!(ok = wait(&ctl->tempty[slot], ((use >> 1) & 1) ^ 1))) break;
+                        if (!(ok = wait_cluster(&ctl->tempty[slot], ((use >> 1) & 1) ^ 1))) break;
                         sm100::tc_fence_after();
                         const bool last = (kb & 1) || kb == P.nkb - 1;
                         if (lead) {
@@ -614,7 +629,9 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
     } else if (wg == 1) {
         sm100::regs_shrink<P_REGS_1>();
         // A look at every scale of this CTA's part of tile number ti, a quarter a
-        // warp, posted to both CTAs.
+        // warp, posted to both CTAs: into this one's shared memory, and to the other
+        // as a word that carries its own signal (cluster-scope releases for it took
+        // 4 % of the whole call: 181 against 173 us).
         auto look = [&](int tile, uint32_t ti) {
             const int row = tile % T.num_m * PBM + (int)rank * 128 + (threadIdx.x & 127), n0 = tile / T.num_m * BN;
             const int wb0 = n0 / KB, words = ((min(n0 + BN, P.N) - 1) / KB - wb0 + 1) * P.nkb;
@@ -628,11 +645,12 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
             const uint32_t any = __any_sync(0xffffffffu, odd), e = ti % RING;
             if (lane == 0) {
                 // the entry's readers of RING tiles ago are done, in both CTAs
-                wait_flag_idle(&ctl->mempty[e], ((ti / RING) & 1) ^ 1, abort_flag, P.flag);
-                for (uint32_t r = 0; r < 2; r++) {
-                    sm100::st_cluster_u32(sm100::map_to_rank(reinterpret_cast<uint32_t*>(&ctl->odd[e][rank]) + q, r), any);
-                    sm100::mbar_arrive_cluster(sm100::map_to_rank(&ctl->mfull[e], r));
-                }
+                wait_flag_idle<true>(&ctl->mgone[e], ((ti / RING) & 1) ^ 1, abort_flag, P.flag);
+                uint32_t* word = reinterpret_cast<uint32_t*>(&ctl->odd[e][rank]) + q;
+                *word = any;
+                if (q == 0) sm100::mbar_arrive_expect_tx(&ctl->mfull[e], 16);
+                sm100::mbar_arrive(&ctl->mfull[e]);
+                sm100::st_async_u32(sm100::map_to_rank(word, rank ^ 1), any, sm100::map_to_rank(&ctl->mfull[e], rank ^ 1));
             }
             __syncwarp();
         };
@@ -692,7 +710,7 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
                 sm100::tmem_wait_st();
                 sm100::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) sm100::mbar_arrive_cluster_cta(sm100::map_to_rank(&ctl->sfull[grp % RING], 0));
+                if (lane == 0) sm100::mbar_arrive_cluster_relaxed(sm100::map_to_rank(&ctl->sfull[grp % RING], 0));
             }
             if (!ok) break;
         }
@@ -753,7 +771,7 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
                         } else {                 // the slot is read: back to the MMA warp
                             sm100::tc_fence_before();
                             __syncwarp();
-                            if (lane == 0) sm100::mbar_arrive_cluster_cta(slot ? tempty[1] : tempty[0]);
+                            if (lane == 0) sm100::mbar_arrive_cluster_relaxed(slot ? tempty[1] : tempty[0]);
                         }
                         const uint32_t sb = __float_as_uint(step(c / 2) ? s1 : s0);
                         const uint64_t ss = pack2(sb, sb);
@@ -780,7 +798,7 @@ k_fp8_linear_pair(const __grid_constant__ CUtensorMap mx, const __grid_constant_
                     if (c == nc - 1) {
                         sm100::tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) sm100::mbar_arrive_cluster_cta((use & 1) ? tempty[1] : tempty[0]);
+                        if (lane == 0) sm100::mbar_arrive_cluster_relaxed((use & 1) ? tempty[1] : tempty[0]);
                     }
                 } else {
                     #pragma unroll

@@ -309,8 +309,11 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t pa
         : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+// A word into another CTA's shared memory that counts 4 bytes on its mbarrier
+// `bar` when it has arrived: whoever has waited for that (cluster scope) sees it.
+__device__ __forceinline__ void st_async_u32(uint32_t cluster_addr, uint32_t v, uint32_t bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];"
+                 ::"r"(cluster_addr), "r"(v), "r"(bar) : "memory");
 }
 // Four floats of another CTA's shared memory (shared::cluster address).
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
@@ -321,12 +324,13 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t cluster_addr) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-// The same with release semantics inside the CTA only: for handing back TMEM
-// that was read (tcgen05.wait::ld has completed the reads), where no written
-// memory has to become visible to the other CTA.  The cluster-scope release
-// above is a memory barrier of about a thousand cycles.
-__device__ __forceinline__ void mbar_arrive_cluster_cta(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+// The same without a release, for handing over TMEM only: PTX orders tcgen05.ld
+// and .st by their wait and the thread-sync fences (tc_fence_before, the arrive,
+// the other side's cluster-scope wait, tc_fence_after), so that the barrier only
+// has to carry the signal.  Memory written before is not published.  (A
+// cluster-scope release is a memory barrier of 1000 to 2500 cycles.)
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // 2-D TMA tile load into this CTA's shared memory whose completion is
 // counted on an mbarrier of either CTA of the pair (`bar_cluster`).

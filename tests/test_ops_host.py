@@ -221,3 +221,33 @@ def test_sizes_past_the_limits_are_refused():
         with pytest.raises(s2b.S2BError) as e:
             s2b.groupnorm_workspace(*sizes)
         assert "more than" in str(e.value)
+
+
+def test_pair_linear_orders_what_crosses_between_its_ctas():
+    """What one CTA of a pair hands to the other, besides TMA and MMA completions: TMEM that it has read or written, as a
+    cluster-scope signal between the fences that order TMEM accesses; a verdict's words, as asynchronous stores that carry
+    their own signal; and, ahead of the next such store, that the verdict's readers are done, as a cluster-scope release.
+    Read from the source: no run shows a missing order."""
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(s2b.__file__))), "csrc")
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, "k_fp8_linear.cu")).read())
+    text = text[text.index("k_fp8_linear_pair("):]
+    assert "st_cluster" not in text
+    remote = re.findall(r"(mbar_arrive_cluster\w*)\(([^;]*)\);", text)
+    relaxed = [a for f, a in remote if f == "mbar_arrive_cluster_relaxed"]
+    release = [a for f, a in remote if f == "mbar_arrive_cluster"]
+    assert len(remote) == len(relaxed) + len(release) == 4
+    assert all("sfull" in a or "tempty" in a for a in relaxed) and all("mgone" in a for a in release), remote
+    for m in re.finditer(r"mbar_arrive_cluster_relaxed", text):
+        assert "tc_fence_before()" in text[m.start() - 200: m.start()]
+    cluster_waits = {"wait_cluster", "wait_flag_idle<true>", "mbar_try_wait_cluster"}
+    for bar in ("sfull", "tempty", "mfull", "mgone"):
+        used = set(re.findall(r"([\w<>]+)\(&ctl->%s\[" % bar, text)) - {"mbar_init", "map_to_rank", "mbar_arrive", "mbar_arrive_expect_tx"}
+        assert used and used <= cluster_waits, (bar, used)
+    # the stores: after the wait for both CTAs' readers
+    post = text[text.index("wait_flag_idle<true>(&ctl->mgone"):]
+    assert post.index("st_async_u32") < 700 and text.count("st_async_u32") == 1
+    assert "map_to_rank(&ctl->mempty" not in text
+    arrive = re.search(r"mbar_arrive_cluster_relaxed\(.*?\n}", open(os.path.join(csrc, "sm100.cuh")).read(), re.S).group(0)
+    assert "mbarrier.arrive.relaxed.cluster.shared::cluster" in arrive
