@@ -77,11 +77,13 @@ int run_op(s2b_ctx* ctx, const Args& a, void* stream) {
         if (!((at.type == cudaMemoryTypeDevice && at.device == dev) || at.type == cudaMemoryTypeManaged))
             return refuse(ctx, S2B_ERR_ARG, "a buffer is not memory of the context's device");
     }
-    cudaGetLastError();                  // an earlier call's error is not this one's
+    // an earlier call's error is not this one's, and stays pending
     const int n = s2b::op_launch(a, (cudaStream_t)stream);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return refuse(ctx, S2B_ERR_CUDA, cudaGetErrorString(e));
-    if (n < 0) return refuse(ctx, S2B_ERR_UNSUPPORTED, "the operator's kernel cannot be launched for this call");
+    if (n == -1) return refuse(ctx, S2B_ERR_UNSUPPORTED, "the operator's kernel cannot be launched for this call");
+    if (n < 0) {
+        cudaGetLastError();              // reported here
+        return refuse(ctx, S2B_ERR_CUDA, cudaGetErrorString((cudaError_t)(-1 - n)));
+    }
     ctx->dit.count_launches(n);
     return S2B_OK;
 }

@@ -322,7 +322,7 @@ int launch_narrow(const Fp8LinearArgs& a, const LinParams& P, cudaStream_t s) {
     int split = 1;
     while (split < 8 && tiles * split * 2 <= 2L * op_sms() && P.nkb >= 4 * split) split *= 2;
     if (tiles * split > 2147483647L) return -1;
-    return launch_chained(k_fp8_linear_narrow<BT>, dim3((unsigned)(tiles * split)), 192, C::SMEM, split, s, mw, mx, P, split) ? 1 : -1;
+    return launch_chained(k_fp8_linear_narrow<BT>, dim3((unsigned)(tiles * split)), 192, C::SMEM, split, s, mw, mx, P, split);
 }
 
 // ---------------------------------------------------------------- many rows
@@ -851,7 +851,7 @@ int launch_pair(const Fp8LinearArgs& a, const LinParams& P, cudaStream_t s) {
     }
     int pairs = op_sms() / 2;
     if (T.total < pairs) pairs = T.total;
-    return launch_chained(k_fp8_linear_pair<BN>, dim3(2 * pairs), PTHREADS, PairCfg8<BN>::SMEM, 0, s, mx, mw, my, P, T) ? 1 : -1;
+    return launch_chained(k_fp8_linear_pair<BN>, dim3(2 * pairs), PTHREADS, PairCfg8<BN>::SMEM, 0, s, mx, mw, my, P, T);
 }
 
 }  // namespace

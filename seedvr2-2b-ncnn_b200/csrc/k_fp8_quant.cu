@@ -281,11 +281,11 @@ int launch(const Fp8QuantArgs& a, cudaStream_t s) {
     if (a.block_rows == 1) {
         const long g = ((kb + QR_BLKS - 1) / QR_BLKS) * ((a.rows + QR_ROWS - 1L) / QR_ROWS);
         if (g > 2147483647L) return -1;
-        return launch_chained(vec ? k_fp8_quant_rows<T, true> : k_fp8_quant_rows<T, false>, dim3((unsigned)g), 256, 0, 0, s, x, a.rows, a.cols, a.ldx, q, a.ldq, a.scale) ? 1 : -1;
+        return launch_chained(vec ? k_fp8_quant_rows<T, true> : k_fp8_quant_rows<T, false>, dim3((unsigned)g), 256, 0, 0, s, x, a.rows, a.cols, a.ldx, q, a.ldq, a.scale);
     }
     const long g = kb * ((a.rows + 127L) / 128);
     if (g > 2147483647L) return -1;
-    return launch_chained(vec ? k_fp8_quant_blocks<T, true> : k_fp8_quant_blocks<T, false>, dim3((unsigned)g), 256, 0, 0, s, x, a.rows, a.cols, a.ldx, q, a.ldq, a.scale) ? 1 : -1;
+    return launch_chained(vec ? k_fp8_quant_blocks<T, true> : k_fp8_quant_blocks<T, false>, dim3((unsigned)g), 256, 0, 0, s, x, a.rows, a.cols, a.ldx, q, a.ldq, a.scale);
 }
 
 }  // namespace

@@ -475,7 +475,7 @@ bool plan_chip(const GroupNormArgs& a, int vec, int xe, GnParams& P, int& rv) {
 }
 
 template <typename TX, typename TY, int VEC, int SUB>
-bool launch_chip(const GnParams& P, int batch, int rv, cudaStream_t s) {
+int launch_chip(const GnParams& P, int batch, int rv, cudaStream_t s) {
     return launch_chained(rv == 4 ? k_gn_chip<TX, TY, VEC, SUB, 4> : k_gn_chip<TX, TY, VEC, SUB, 16>,
                           dim3((unsigned)((long)batch * P.slabs * P.split)), THREADS, 0, P.split, s, P);
 }
@@ -483,7 +483,7 @@ bool launch_chip(const GnParams& P, int batch, int rv, cudaStream_t s) {
 template <typename TX, typename TY, int VEC, int SUB>
 int launch_v(const GroupNormArgs& a, GnParams& P, cudaStream_t s) {
     int rv;
-    if (plan_chip(a, VEC, sizeof(TX), P, rv)) return launch_chip<TX, TY, VEC, SUB>(P, a.batch, rv, s) ? 1 : -1;
+    if (plan_chip(a, VEC, sizeof(TX), P, rv)) return launch_chip<TX, TY, VEC, SUB>(P, a.batch, rv, s);
     const int vecs = P.C / VEC;
     P.tiles = (vecs + tile_cols(vecs) - 1) / tile_cols(vecs);
     if (P.tiles > 65535) return -1;
@@ -494,10 +494,10 @@ int launch_v(const GroupNormArgs& a, GnParams& P, cudaStream_t s) {
     P.stat = (float4*)a.work;
     P.part = P.stat + (size_t)a.batch * P.G;
     const dim3 g(P.chunks, P.tiles, a.batch), ga((a.rows + achunk - 1) / achunk, P.tiles, a.batch);
-    if (!launch_chained(k_gn_stats<TX, VEC, SUB>, g, THREADS, 0, 0, s, P)) return -1;
-    if (!launch_chained(k_gn_join, dim3(P.G, a.batch), 128, 0, 0, s, P)) return -1;
-    if (!launch_chained(k_gn_apply<TX, TY, VEC, SUB>, ga, THREADS, 0, 0, s, P)) return -1;
-    return 3;
+    int n = launch_chained(k_gn_stats<TX, VEC, SUB>, g, THREADS, 0, 0, s, P);
+    if (n > 0) n = launch_chained(k_gn_join, dim3(P.G, a.batch), 128, 0, 0, s, P);
+    if (n > 0) n = launch_chained(k_gn_apply<TX, TY, VEC, SUB>, ga, THREADS, 0, 0, s, P);
+    return n > 0 ? 3 : n;
 }
 
 template <typename TX, typename TY>

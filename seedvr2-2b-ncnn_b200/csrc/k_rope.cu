@@ -260,7 +260,7 @@ int launch_hu(RopeParams& P, long ctas, cudaStream_t s) {
     P.chunks = batches / P.passes;
     const long g = ctas * P.chunks;
     if (g > 2147483647L) return -1;
-    return launch_chained(P.p.half ? k_rope<T, VEC, true, HU> : k_rope<T, VEC, false, HU>, dim3((unsigned)g), 256, 0, 0, s, P) ? 1 : -1;
+    return launch_chained(P.p.half ? k_rope<T, VEC, true, HU> : k_rope<T, VEC, false, HU>, dim3((unsigned)g), 256, 0, 0, s, P);
 }
 
 template <typename T, int VEC>

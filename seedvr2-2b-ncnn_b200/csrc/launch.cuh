@@ -21,9 +21,10 @@ __device__ __forceinline__ void chain_begin() {
     chain_wait();
 }
 
-// True when the launch was accepted.  cluster: CTAs a cluster (0: none).
+// 1 (kernel launched), or -1 - the CUDA error that refused it.  cluster: CTAs a
+// cluster (0: none).
 template <typename... P, typename... A>
-bool launch_chained(void (*f)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t s, const A&... args) {
+int launch_chained(void (*f)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t s, const A&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
@@ -36,7 +37,8 @@ bool launch_chained(void (*f)(P...), dim3 grid, int threads, size_t smem, int cl
     at[1].val.clusterDim.x = cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = cluster ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, f, static_cast<P>(args)...) == cudaSuccess;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, f, static_cast<P>(args)...);
+    return e == cudaSuccess ? 1 : -1 - (int)e;
 }
 
 }  // namespace s2b

@@ -58,7 +58,8 @@ inline OpPtrs op_ptrs(const RopeArgs& a) { return {{a.x, a.y, a.pos}, 3}; }
 inline OpPtrs op_ptrs(const GroupNormArgs& a) { return {{a.x, a.y, a.work, a.gamma, a.beta}, 5}; }
 
 // Enqueue on s, on the current device; returns the number of kernels
-// launched, or -1 when the launch could not be set up.
+// launched, -1 when the launch could not be set up, or -1 - the CUDA error of a
+// launch that was refused.
 int op_launch(const Fp8QuantArgs& a, cudaStream_t s);
 int op_launch(const Fp8LinearArgs& a, cudaStream_t s);
 int op_launch(const RopeArgs& a, cudaStream_t s);

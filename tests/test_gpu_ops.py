@@ -854,3 +854,22 @@ def test_rope_many_tokens_and_wide_heads(ctx, t, T, H, D, kw):
     assert (y[-64:] == 55).all()
     run_rope(ctx, plan, x, t, None, 0, 7, x)
     assert torch.equal(x, y[:-64].view(1, T, H, D))
+
+
+# ---------------------------------------------------------------- errors that are not a call's
+def test_pending_cuda_error_stays_the_callers(tmp_path):
+    """A CUDA error left pending before an operator call is still there after it, and the call succeeds."""
+    import glob
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    objs = glob.glob(os.path.join(root, "seedvr2-2b-ncnn_b200", "build", "*.o"))
+    if not objs:
+        pytest.skip("the library's objects are not here")
+    exe = str(tmp_path / "pending_error")
+    r = subprocess.run(["g++", "-std=c++17", "-O1", "-I", os.path.join(root, "include"), "-I/usr/local/cuda/include",
+                        os.path.join(root, "tests", "cpp", "pending_error.cpp"), *objs, "-L/usr/local/cuda/lib64", "-lcudart_static", "-lpthread",
+                        "-ldl", "-lrt", "-o", exe], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    r = subprocess.run([exe], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout == "ok\n", r.stderr
