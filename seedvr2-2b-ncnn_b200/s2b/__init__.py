@@ -468,7 +468,7 @@ class DitB200:
     def fp8_quant_dev(self, d_x: int, x_type: int, rows: int, cols: int, ldx: int, block_rows: int, d_q: int, ldq: int,
                       d_scale: int, stream: int):
         """e4m3 codes and scales of x in blocks of 128 columns x 1 or 128 rows (s2b_fp8_quant_dev)."""
-        rc = self._op(_QUANT.pack(0, self._h, stream, d_x or 0, x_type, rows, cols, ldx, block_rows, d_q or 0, ldq,
+        rc = self._op(_QUANT.pack(0, self._h, stream or 0, d_x or 0, x_type, rows, cols, ldx, block_rows, d_q or 0, ldq,
                                   d_scale or 0))
         if rc:
             self._c(rc)
@@ -476,7 +476,7 @@ class DitB200:
     def linear_fp8_dev(self, d_xq: int, ldx: int, d_xs: int, M: int, K: int, d_wq: int, ldw: int, d_ws: int, N: int,
                        d_bias, d_y: int, y_type: int, ldy: int, stream: int):
         """y = (xq . xs) (wq . ws)^T (+ bias) on 8-bit codes (s2b_linear_fp8_dev)."""
-        rc = self._op(_LINEAR.pack(1, self._h, stream, d_xq or 0, ldx, d_xs or 0, M, K, d_wq or 0, ldw, d_ws or 0, N,
+        rc = self._op(_LINEAR.pack(1, self._h, stream or 0, d_xq or 0, ldx, d_xs or 0, M, K, d_wq or 0, ldw, d_ws or 0, N,
                                    d_bias or 0, d_y or 0, y_type, ldy))
         if rc:
             self._c(rc)
@@ -484,7 +484,11 @@ class DitB200:
     def rope_dev(self, plan: s2b_rope, d_x: int, x_type: int, batch: int, tokens: int, heads: int, head_dim: int,
                  x_strides, d_pos, pos_batch_stride: int, pos0: int, d_y: int, y_strides, inverse: bool, stream: int):
         """Rotary positions (s2b_rope_dev); strides are (batch, token, head) in elements."""
-        rc = self._op(_ROPE.pack(2, self._h, stream, ctypes.addressof(plan), d_x or 0, x_type, batch, tokens, heads,
+        if not isinstance(plan, s2b_rope):
+            raise TypeError("plan is one that rope_plan made")
+        if len(x_strides) != 3 or len(y_strides) != 3:
+            raise ValueError("x_strides and y_strides are (batch, token, head)")
+        rc = self._op(_ROPE.pack(2, self._h, stream or 0, ctypes.addressof(plan), d_x or 0, x_type, batch, tokens, heads,
                                  head_dim, *x_strides, d_pos or 0, pos_batch_stride, pos0, d_y or 0, *y_strides,
                                  1 if inverse else 0))
         if rc:
@@ -494,7 +498,7 @@ class DitB200:
                       d_beta, eps: float, act: int, d_y: int, y_type: int, ldy: int, d_work, work_bytes: int,
                       stream: int):
         """GroupNorm (+ SiLU) over channel-last rows (s2b_groupnorm_dev)."""
-        rc = self._op(_NORM.pack(3, self._h, stream, d_x or 0, x_type, batch, rows, channels, ldx, groups, d_gamma or 0,
+        rc = self._op(_NORM.pack(3, self._h, stream or 0, d_x or 0, x_type, batch, rows, channels, ldx, groups, d_gamma or 0,
                                  d_beta or 0, eps, act, d_y or 0, y_type, ldy, d_work or 0, work_bytes))
         if rc:
             self._c(rc)

@@ -251,3 +251,25 @@ def test_pair_linear_orders_what_crosses_between_its_ctas():
     assert "map_to_rank(&ctl->mempty" not in text
     arrive = re.search(r"mbar_arrive_cluster_relaxed\(.*?\n}", open(os.path.join(csrc, "sm100.cuh")).read(), re.S).group(0)
     assert "mbarrier.arrive.relaxed.cluster.shared::cluster" in arrive
+
+
+def test_python_calls_check_what_they_pack():
+    """The short calls pack their arguments themselves: None is the default stream as in the other methods, strides are
+    three, and a plan is one that rope_plan made."""
+    c = s2b.DitB200.__new__(s2b.DitB200)
+    c._ctx, c._h, c._op = ctypes.c_void_p(), 0, s2b.lib().s2b_op_packed
+    plan, st = s2b.rope_plan([64]), (1536, 512, 128)
+    calls = [lambda s: c.fp8_quant_dev(X, BF16, 4, 256, 256, 1, Q, 256, S, s),
+             lambda s: c.linear_fp8_dev(X, 256, S, 4, 256, W, 256, V, 64, None, Y, BF16, 64, s),
+             lambda s: c.rope_dev(plan, X, BF16, 2, 3, 4, 128, st, None, 0, 0, Y, st, False, s),
+             lambda s: c.groupnorm_dev(X, BF16, 2, 10, 64, 64, 8, S, V, 1e-6, 1, Y, BF16, 64, B, 1 << 19, s)]
+    for call in calls:
+        for s in (0, None):
+            with pytest.raises(s2b.S2BError, match="null context"):
+                call(s)
+    for xs, ys in ((st[:2], st), (st, st + (1,)), (st + (1,), st[:2]), ((), st * 2)):
+        with pytest.raises(ValueError, match="strides"):
+            c.rope_dev(plan, X, BF16, 2, 3, 4, 128, xs, None, 0, 0, Y, ys, False, 0)
+    for p in (None, s2b.s2b_rope_config(), ctypes.c_int(0)):
+        with pytest.raises(TypeError, match="rope_plan"):
+            c.rope_dev(p, X, BF16, 2, 3, 4, 128, st, None, 0, 0, Y, st, False, 0)
