@@ -295,6 +295,23 @@ def test_linear_same_bits_every_time_and_on_two_streams(ctx):
         assert torch.equal(y.view(torch.int16), alone[i].view(torch.int16))
 
 
+@pytest.mark.parametrize("K", [2560, 5120, 6912])
+@pytest.mark.parametrize("M,N", [(1, 512), (40, 768), (1536, 1280)])
+def test_linear_error_against_the_norm_of_y(ctx, M, N, K):
+    """What the header promises of fp32 outputs, against y's norm.  Scales that are no powers of two, and few rows: a
+    block's sum is cut at most four times (2^-23 of it: 4.8e-7 at the very most, half that on average) and added with a
+    rounding (2^-24 * sqrt(blocks / 2) against independent blocks, 3.1e-7 at the most, 1.8e-7 in rms): 5e-7.  Powers of
+    two in the CTA-pair kernel: the tensor core's accumulator takes all of K, cut at each 32 codes: 2e-6, a quarter of what
+    24 bits would lose.  Sums held in 16 bits anywhere would be off by 1e-3."""
+    g = gen(K + M)
+    xq, xs = codes(normal(g, M, K) * torch.exp(0.5 * normal(g, M, 1)), 1)
+    wq, ws = codes(0.02 * normal(g, N, K), 128)
+    for a, b, bound in ((xs, ws, 2e-6 if M > 1000 else 5e-7), (xs * 1.1, ws * 0.7, 5e-7)):
+        ref, _ = linear64(xq, a, wq, b, K, None)
+        y = run_linear(ctx, xq, a, wq, b, K, None, FP32)[:M].double()
+        assert ((y - ref).norm() / ref.norm()).item() <= bound
+
+
 def test_linear_error_flag_reaches_check_errors():
     c = s2b.DitB200(0, s2b.PREC_BF16)
     try:
