@@ -342,8 +342,10 @@ int s2b_rope_plan(const s2b_rope_config* config, s2b_rope* plan);
  * t * axes + a] (int32, any value; stride 0 shares them between samples), or
  * pos0 + t on every axis when d_pos is NULL.  y may be x with the same strides;
  * otherwise the two, from first to last value, must not overlap.  No buffer
- * may reach over more than 2^40 values.  Angles are exact to 2^-32 of a turn at
- * every position. */
+ * may reach over more than 2^40 values.  A position's fraction of a turn is an
+ * integer product, exact to 2^-32 at every position, and rounded once, to fp32:
+ * the angle whose sine and cosine are taken is off by at most 2^-26 + 2^-31 of a
+ * turn (1e-7 rad). */
 int s2b_rope_dev(s2b_ctx* ctx, const s2b_rope* plan, const void* d_x, int type, int batch, int tokens, int heads,
                  int head_dim, const long x_strides[3], const int* d_pos, long pos_batch_stride, int pos0, void* d_y,
                  const long y_strides[3], int inverse, void* stream);

@@ -93,7 +93,8 @@ __device__ __forceinline__ float2 rotate(float a, float d, float2 cs) {
 __device__ __forceinline__ float2 turn(const RopeParams& P, const SharedPlan& S, int i, const int* pos, int t) {
     const int64_t p = pos ? (int64_t)pos[S.axis[i]] : (int64_t)P.pos0 + t;
     const uint64_t f = (uint64_t)p * S.turns[i];         // wraps whole turns away
-    // top 32 bits as a signed fraction of half a turn in [-1, 1)
+    // top 32 bits as a signed fraction of half a turn in [-1, 1), rounded to fp32:
+    // by up to 2^-26 of a turn next to half a turn
     const float half = (float)(int32_t)(f >> 32) * 4.656612873077393e-10f;
     float2 r;
     sincospif(half, &r.y, &r.x);

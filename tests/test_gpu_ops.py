@@ -445,6 +445,21 @@ def test_rope_far_positions(ctx):
     assert ((z[:, 1].double() - ref).abs() <= 13 * 2.0 ** -24 * mag[:, 1]).all()
 
 
+def test_rope_angles_are_as_exact_as_documented(ctx):
+    """Pairs (1, 0) become (cos, sin) of the angle: off by the documented 2^-26 + 2^-31 of a turn and by 2 ulp (2^-24 each
+    below 1) of the sine or cosine, anywhere in 32 bits; the multiplications by 1 and 0 are exact."""
+    plan = s2b.rope_plan([256], layout="interleaved", theta=500.0)
+    g = gen(6)
+    ps = [0, 1, -1, 2 ** 31 - 1, -(2 ** 31)] + torch.randint(-(2 ** 31), 2 ** 31, (300,), generator=g, device=DEV).tolist()
+    x = torch.zeros(1, len(ps), 1, 256, device=DEV)
+    x[..., ::2] = 1
+    pos = torch.tensor(ps, dtype=torch.int32, device=DEV).view(1, -1, 1)
+    y = run_rope(ctx, plan, x, FP32, pos, 0, 0, torch.empty_like(x))[0, :, 0].double()
+    ang = torch.tensor([[(p * plan.turns[i] % 2 ** 64) / 2.0 ** 64 * 2 * math.pi for i in range(128)] for p in ps], dtype=torch.float64, device=DEV)
+    tol = 2 * math.pi * (2.0 ** -26 + 2.0 ** -31) + 2 * 2.0 ** -24
+    assert (y[:, ::2] - ang.cos()).abs().max().item() <= tol and (y[:, 1::2] - ang.sin()).abs().max().item() <= tol
+
+
 def test_rope_inverse_is_the_gradient(ctx):
     """<rope(x), w> differs by <inverse(w), d> along d: the map is linear, so the difference is exact but for rounding."""
     plan = s2b.rope_plan([64], layout="half", scaling="yarn", factor=4.0, original_length=1000)
