@@ -795,6 +795,29 @@ def test_host_memory_is_refused_and_writes_nothing(ctx):
     assert not h.any() and not d.any() and not q.any() and not pinned.any()
 
 
+def test_host_memory_is_refused_with_its_code(ctx):
+    """Each operator with one buffer on the host, pageable or page-locked: the argument code, whatever the words."""
+    d = torch.zeros(64, 128, device=DEV)
+    q, s = torch.zeros(64, 128, dtype=torch.uint8, device=DEV), torch.zeros(64, device=DEV)
+    plan, n = s2b.rope_plan([128]), 1 << 14
+    for h in (torch.zeros(64, 128), torch.zeros(64, 128).pin_memory()):
+        p = h.data_ptr()
+        calls = [lambda: ctx.fp8_quant_dev(p, FP32, 16, 128, 128, 1, q.data_ptr(), 128, s.data_ptr(), stream()),
+                 lambda: ctx.fp8_quant_dev(d.data_ptr(), FP32, 16, 128, 128, 1, p, 128, s.data_ptr(), stream()),
+                 lambda: ctx.linear_fp8_dev(q.data_ptr(), 128, p, 16, 128, q.data_ptr(), 128, s.data_ptr(), 16, None, d.data_ptr(), FP32, 128, stream()),
+                 lambda: ctx.linear_fp8_dev(q.data_ptr(), 128, s.data_ptr(), 16, 128, q.data_ptr(), 128, s.data_ptr(), 16, None, p, FP32, 128, stream()),
+                 lambda: ctx.rope_dev(plan, p, FP32, 1, 16, 1, 128, (0, 128, 0), None, 0, 0, d.data_ptr(), (0, 128, 0), False, stream()),
+                 lambda: ctx.rope_dev(plan, d.data_ptr(), FP32, 1, 16, 1, 128, (0, 128, 0), p, 0, 0, d.data_ptr(), (0, 128, 0), False, stream()),
+                 lambda: ctx.groupnorm_dev(d.data_ptr(), FP32, 1, 16, 128, 128, 8, None, p, 1e-6, 0, d.data_ptr(), FP32, 128, q.data_ptr(), n, stream()),
+                 lambda: ctx.groupnorm_dev(d.data_ptr(), FP32, 1, 16, 128, 128, 8, None, None, 1e-6, 0, d.data_ptr(), FP32, 128, p, n, stream())]
+        for c in calls:
+            with pytest.raises(s2b.S2BError) as e:
+                c()
+            assert e.value.code == 1
+        torch.cuda.synchronize()
+        assert not h.any() and not d.any() and not q.any() and not s.any()
+
+
 def test_empty_calls_write_nothing(ctx):
     y = torch.full((4, 128), 5.0, device=DEV)
     plan = s2b.rope_plan([128])
