@@ -74,8 +74,8 @@ __device__ __forceinline__ void store_y(void* y, int t, size_t i, float v) {
 // workspace), so that few tiles still stream the weights from every SM.
 // Bound by latency: of the 6.5 us that a CTA takes for 58 rows x 5120 x 2560
 // (13.7 MB), 1.4 pass before the first block has arrived, 2 in five blocks, 3 in
-// joining eight ranks.  B200: that call 9.8 us, 1 x 2560 x 7680 7.0 us, the
-// smallest call 5.2 us.
+// joining eight ranks.  B200, in a burst: that call 9.5 us, 1 x 2560 x 7680 6.6 us,
+// the smallest call 5.2 us.
 template <int BT> struct NarrowCfg {
     static constexpr int W_BYTES = 128 * KB, X_BYTES = BT * KB, STAGE = W_BYTES + X_BYTES;
     static constexpr int STAGES = BT == 64 ? 4 : 5;
@@ -864,8 +864,8 @@ int op_launch(const Fp8LinearArgs& a, cudaStream_t s) {
     if (!P.flag) return -1;
     // The narrow kernel while its tiles are few enough for four ranks or more
     // along K at two CTAs an SM; past that the pair kernel even where it leaves
-    // SMs idle (K 2560, N 2560: 192 rows 14.3 against 15.0 us, 256 rows 21.7
-    // against 15.1).
+    // SMs idle (K 2560, N 2560, in a burst: 192 rows 9.6 against 11.6 us, 256 rows
+    // 11.9 against 11.8).
     const long narrow = ((a.N + 127L) / 128) * ((a.M + 63L) / 64);
     if (a.M > 64 && 4 * narrow > 2L * op_sms()) {
         // The tile width with the cheaper waves: a 192-column tile takes 0.94 of

@@ -14,9 +14,9 @@
 // where only 16 of 64 pairs turn, every warp waits for the few threads that
 // turn, 147 us against 99 for 8 heads of 131042 tokens in bf16; 25 against 20
 // for the grid below.)  Chunks of heads are neighbouring CTAs, so the CTAs
-// together walk through memory in order.  B200: 40 heads of 128 at 5440 tokens
-// in bf16 (111 MB) 19.8 us; 8 heads of 128 at 131042 tokens in fp32 (1.07 GB)
-// 169 us, 6.4 TB/s.
+// together walk through memory in order.  B200, in a burst: 40 heads of 128 at
+// 5440 tokens in bf16 (111 MB) 19.8 us; 8 heads of 128 at 131042 tokens in fp32
+// (1.07 GB) 170 us, 6.3 TB/s (176 to 182 in a long run).
 #include "kcommon.cuh"
 #include "launch.cuh"
 #include "ops.h"
