@@ -355,7 +355,8 @@ int s2b_rope_dev(s2b_ctx* ctx, const s2b_rope* plan, const void* d_x, int type, 
  * with the mean and (biased) variance over the rows and the channels / groups
  * adjacent channels of group g of one sample; statistics in fp32, about running
  * means, so that neither a mean far from zero nor single values far off cost
- * accuracy (the squared deviations' sum has to stay below fp32's 3.4e38).  x is
+ * accuracy.  (Where the squared deviations' sum of a group of finite values
+ * passes fp32's 3.4e38, its variance is infinite and y act(beta).)  x is
  * (batch, rows, channels) with row pitch ldx (samples adjacent), y likewise
  * with ldy; gamma, beta (channels) fp32 or NULL (1, 0).  y may be x with the
  * same type and pitch; otherwise they must not overlap.  d_work: device

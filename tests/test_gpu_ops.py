@@ -561,6 +561,23 @@ def test_groupnorm_silu_over_its_whole_range(ctx, t, S):
     assert (err <= tol).all(), ((err / tol).max().item(), beta[(err / tol).amax(dim=(0, 1)).argmax()].item())
 
 
+@pytest.mark.parametrize("S,C,G", [(40, 64, 8), (20000, 64, 8), (300, 10, 2), (30000, 60, 20)])
+@pytest.mark.parametrize("t", [FP32, BF16], ids=IDS)
+def test_groupnorm_squares_past_fp32(ctx, t, S, C, G):
+    """Finite values whose squared deviations leave fp32: the variance is infinite, as in plain fp32 statistics, and y is
+    act(beta) in that group; the other groups are what they are without it."""
+    g = gen(S)
+    x, beta = normal(g, 1, S, C).to(DT[t]), normal(g, C)
+    ref = run_norm(ctx, x, G, None, beta, 1e-6, False, FP32)
+    for rows in ([0], [S - 1], list(range(0, S, 3)), [S // 2, S // 2 + 1]):
+        z = x.clone()
+        z[0, rows, 0] = 1e25
+        if len(rows) == 2:
+            z[0, rows[1], 0] = -1e25
+        y = run_norm(ctx, z, G, None, beta, 1e-6, False, FP32)
+        assert torch.equal(y[..., : C // G], beta[: C // G].expand(1, S, -1)) and torch.equal(y[..., C // G:], ref[..., C // G:])
+
+
 def test_groupnorm_nan_and_inf_stay_in_their_group(ctx):
     g = gen(12)
     x = normal(g, 2, 900, 64)
